@@ -1,0 +1,80 @@
+// ecnf_attention.hip — launches of the cross attention kernels (context_attention.hpp) for one element type:
+// ECNF_ATT_TYPE 0 fp32, 1 bf16, 2 fp16 (one translation unit each).
+#include "context_attention.hpp"
+
+namespace ecnf_ctx {
+namespace {
+
+#if ECNF_ATT_TYPE == 0
+typedef float T;
+#define ECNF_ATT_NAME(x) x##_f32
+#elif ECNF_ATT_TYPE == 1
+typedef __bf16 T;
+#define ECNF_ATT_NAME(x) x##_bf16
+#else
+typedef _Float16 T;
+#define ECNF_ATT_NAME(x) x##_f16
+#endif
+
+template <class K>
+hipError_t launch(K kernel, int64_t grid, int lds, const Att& a, hipStream_t s) {
+  if (!grid) return hipSuccess;   // no rows or no keys
+  if (lds > 65536) {
+    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+    if (e != hipSuccess) return e;
+  }
+  kernel<<<dim3((unsigned)grid), dim3(256), lds, s>>>(a);
+  return hipGetLastError();
+}
+
+Att with_plan(Att a, const Plan& p, float* part) {
+  a.tiles = p.tiles;
+  a.splits = p.splits;
+  a.part = part;
+  a.part_lse = part + p.part;
+  return a;
+}
+
+template <int DP>
+hipError_t fwd(const Att& in, hipStream_t s) {
+  const Plan p = plan_fwd(in);
+  const Att a = with_plan(in, p, in.part);
+  hipError_t e = p.narrow ? launch(att_fwd<T, DP, 1, 4, 32>, p.grid, FwdShape<T, DP, 1, 4, 32>::kLds, a, s)
+                          : launch(att_fwd<T, DP, 4, 1, 64>, p.grid, FwdShape<T, DP, 4, 1, 64>::kLds, a, s);
+  if (e != hipSuccess || p.splits == 1) return e;
+  const int64_t n = (int64_t)a.C * a.Hk * a.R * (a.D / 4);
+  att_fwd_join<T><<<dim3((unsigned)((n + 255) / 256)), dim3(256), 0, s>>>(a);
+  return hipGetLastError();
+}
+
+template <int DP>
+hipError_t grad(const Att& in, hipStream_t s) {
+  const Plan p = plan_dq(in), y = plan_dkv(in);
+  Att a = with_plan(in, p, in.part);
+  hipError_t e = p.narrow ? launch(att_dq<T, DP, 1, 4, 32>, p.grid, FwdShape<T, DP, 1, 4, 32>::kLds, a, s)
+                          : launch(att_dq<T, DP, 4, 1, 64>, p.grid, FwdShape<T, DP, 4, 1, 64>::kLds, a, s);
+  if (e != hipSuccess) return e;
+  if (p.splits > 1) {
+    const int64_t n = (int64_t)a.C * a.Hk * a.R * (a.D / 4);
+    att_grad_join<T><<<dim3((unsigned)((n + 255) / 256)), dim3(256), 0, s>>>(a, 0);
+    if ((e = hipGetLastError()) != hipSuccess) return e;
+  }
+  a = with_plan(in, y, in.part);
+  e = y.narrow ? launch(att_dkv<T, DP, 1, 4>, y.grid, DkvShape<T, DP, 1, 4>::kLds, a, s)
+               : launch(att_dkv<T, DP, 4, 1>, y.grid, DkvShape<T, DP, 4, 1>::kLds, a, s);
+  if (e != hipSuccess || y.splits == 1) return e;
+  const int64_t n = (int64_t)a.C * a.Hk * a.Lk * (a.D / 4);
+  att_grad_join<T><<<dim3((unsigned)((n + 255) / 256), 2), dim3(256), 0, s>>>(a, 1);
+  return hipGetLastError();
+}
+
+}  // namespace
+
+hipError_t ECNF_ATT_NAME(launch_fwd)(const Att& a, hipStream_t s) {
+  return a.D <= 32 ? fwd<32>(a, s) : a.D <= 64 ? fwd<64>(a, s) : fwd<128>(a, s);
+}
+hipError_t ECNF_ATT_NAME(launch_grad)(const Att& a, hipStream_t s) {
+  return a.D <= 32 ? grad<32>(a, s) : a.D <= 64 ? grad<64>(a, s) : grad<128>(a, s);
+}
+
+}  // namespace ecnf_ctx

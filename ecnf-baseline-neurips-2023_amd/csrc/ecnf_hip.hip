@@ -933,7 +933,7 @@ const char* ecnf_last_error(void) { return g_err.c_str(); }
 
 int ecnf_struct_layout(int32_t which, size_t* out, int32_t cap) {
 #define L_(T, f) offsetof(T, f)
-  size_t v[16];
+  size_t v[32];
   int n = 0;
   switch (which) {
     case 0: {
@@ -967,6 +967,40 @@ int ecnf_struct_layout(int32_t which, size_t* out, int32_t cap) {
       const size_t o[] = {sizeof(ecnf_adam_opts), L_(ecnf_adam_opts, lr), L_(ecnf_adam_opts, b1),
                           L_(ecnf_adam_opts, b2), L_(ecnf_adam_opts, eps), L_(ecnf_adam_opts, eps_root),
                           L_(ecnf_adam_opts, count), L_(ecnf_adam_opts, ema_beta)};
+      n = sizeof(o) / sizeof(o[0]);
+      std::memcpy(v, o, sizeof(o));
+      break;
+    }
+    case 4: {
+      const size_t o[] = {sizeof(ecnf_qk_side), L_(ecnf_qk_side, x), L_(ecnf_qk_side, grad), L_(ecnf_qk_side, out),
+                          L_(ecnf_qk_side, weight), L_(ecnf_qk_side, weight_grad), L_(ecnf_qk_side, positions),
+                          L_(ecnf_qk_side, x_stride), L_(ecnf_qk_side, grad_stride),
+                          L_(ecnf_qk_side, position_stride), L_(ecnf_qk_side, batch), L_(ecnf_qk_side, length),
+                          L_(ecnf_qk_side, heads), L_(ecnf_qk_side, position_type)};
+      n = sizeof(o) / sizeof(o[0]);
+      std::memcpy(v, o, sizeof(o));
+      break;
+    }
+    case 5: {
+      const size_t o[] = {sizeof(ecnf_qk_norm), L_(ecnf_qk_norm, q), L_(ecnf_qk_norm, k), L_(ecnf_qk_norm, dtype),
+                          L_(ecnf_qk_norm, head_dim), L_(ecnf_qk_norm, n_axes), L_(ecnf_qk_norm, axes),
+                          L_(ecnf_qk_norm, interleaved), L_(ecnf_qk_norm, device), L_(ecnf_qk_norm, eps),
+                          L_(ecnf_qk_norm, theta)};
+      n = sizeof(o) / sizeof(o[0]);
+      std::memcpy(v, o, sizeof(o));
+      break;
+    }
+    case 6: {
+      const size_t o[] = {sizeof(ecnf_attention), L_(ecnf_attention, q), L_(ecnf_attention, k), L_(ecnf_attention, v),
+                          L_(ecnf_attention, out), L_(ecnf_attention, out_grad), L_(ecnf_attention, lse),
+                          L_(ecnf_attention, q_grad), L_(ecnf_attention, k_grad), L_(ecnf_attention, v_grad),
+                          L_(ecnf_attention, query_lengths), L_(ecnf_attention, context_lengths),
+                          L_(ecnf_attention, context_mask), L_(ecnf_attention, q_stride),
+                          L_(ecnf_attention, k_stride), L_(ecnf_attention, v_stride),
+                          L_(ecnf_attention, out_grad_stride), L_(ecnf_attention, dtype), L_(ecnf_attention, batch),
+                          L_(ecnf_attention, context_batch), L_(ecnf_attention, n_queries),
+                          L_(ecnf_attention, context_length), L_(ecnf_attention, heads), L_(ecnf_attention, kv_heads),
+                          L_(ecnf_attention, head_dim), L_(ecnf_attention, device), L_(ecnf_attention, scale)};
       n = sizeof(o) / sizeof(o[0]);
       std::memcpy(v, o, sizeof(o));
       break;

@@ -28,9 +28,13 @@ EXPORTED_SYMBOLS = (
     "ecnf_adam_update", "ecnf_update_params", "ecnf_integrate_workspace_size", "ecnf_integrate_ws",
     "ecnf_reserve_workspace", "ecnf_set_exact_form", "ecnf_struct_layout", "ecnf_trainer_set_reduction_arena",
     "ecnf_set_team", "ecnf_team_workgroups", "ecnf_integrate_plan",
+    "ecnf_qk_norm_rotary", "ecnf_qk_norm_workspace_size", "ecnf_qk_norm_rotary_grad",
+    "ecnf_cross_attention_workspace_size", "ecnf_cross_attention", "ecnf_cross_attention_grad",
 )
 
 TARGET_LJ, TARGET_DW = 0, 1
+DTYPE_F32, DTYPE_BF16, DTYPE_F16 = 0, 1, 2
+POS_I32, POS_I64, POS_F32 = 0, 1, 2
 
 
 class EcnfCfg(ctypes.Structure):
@@ -91,14 +95,68 @@ class EcnfAdamOpts(ctypes.Structure):
     ]
 
 
+class EcnfQkSide(ctypes.Structure):
+    _fields_ = [
+        ("x", ctypes.c_void_p),
+        ("grad", ctypes.c_void_p),
+        ("out", ctypes.c_void_p),
+        ("weight", ctypes.c_void_p),
+        ("weight_grad", ctypes.c_void_p),
+        ("positions", ctypes.c_void_p),
+        ("x_stride", ctypes.c_int64 * 3),
+        ("grad_stride", ctypes.c_int64 * 3),
+        ("position_stride", ctypes.c_int64 * 2),
+        ("batch", ctypes.c_int32),
+        ("length", ctypes.c_int32),
+        ("heads", ctypes.c_int32),
+        ("position_type", ctypes.c_int32),
+    ]
+
+
+class EcnfQkNorm(ctypes.Structure):
+    _fields_ = [
+        ("q", EcnfQkSide),
+        ("k", EcnfQkSide),
+        ("dtype", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32),
+        ("n_axes", ctypes.c_int32),
+        ("axes", ctypes.c_int32 * 4),
+        ("interleaved", ctypes.c_int32),
+        ("device", ctypes.c_int32),
+        ("eps", ctypes.c_float),
+        ("theta", ctypes.c_double),
+    ]
+
+
+class EcnfAttention(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_void_p) for n in (
+        "q", "k", "v", "out", "out_grad", "lse", "q_grad", "k_grad", "v_grad", "query_lengths", "context_lengths",
+        "context_mask")] + [
+        ("q_stride", ctypes.c_int64 * 3),
+        ("k_stride", ctypes.c_int64 * 3),
+        ("v_stride", ctypes.c_int64 * 3),
+        ("out_grad_stride", ctypes.c_int64 * 3),
+        ("dtype", ctypes.c_int32),
+        ("batch", ctypes.c_int32),
+        ("context_batch", ctypes.c_int32),
+        ("n_queries", ctypes.c_int32),
+        ("context_length", ctypes.c_int32),
+        ("heads", ctypes.c_int32),
+        ("kv_heads", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32),
+        ("device", ctypes.c_int32),
+        ("scale", ctypes.c_float),
+    ]
+
+
 # the ABI structs in ecnf_struct_layout's `which` order
-ABI_STRUCTS = (EcnfCfg, EcnfSolveOpts, EcnfTarget, EcnfAdamOpts)
+ABI_STRUCTS = (EcnfCfg, EcnfSolveOpts, EcnfTarget, EcnfAdamOpts, EcnfQkSide, EcnfQkNorm, EcnfAttention)
 
 
 def struct_layout(which: int):
     """(sizeof, [field offsets]) of ABI struct `which` as the compiled library lays it out."""
-    buf = (ctypes.c_size_t * 16)()
-    n = load().ecnf_struct_layout(which, buf, 16)
+    buf = (ctypes.c_size_t * 32)()
+    n = load().ecnf_struct_layout(which, buf, 32)
     if n < 0:
         raise ValueError(f"unknown struct {which}")
     return buf[0], list(buf[1:1 + n])
@@ -160,6 +218,13 @@ def load(path: Optional[str] = None) -> ctypes.CDLL:
         "ecnf_integrate_plan": ([P, ctypes.POINTER(EcnfSolveOpts), I32, ctypes.POINTER(I32), ctypes.POINTER(I32)],
                                 ctypes.c_int),
         "ecnf_struct_layout": ([I32, ctypes.POINTER(SZ), I32], ctypes.c_int),
+        # the context operators' argument structs are passed as packed bytes (ecnf_amd.context)
+        "ecnf_qk_norm_rotary": ([P, P], ctypes.c_int),
+        "ecnf_qk_norm_workspace_size": ([P, ctypes.POINTER(SZ)], ctypes.c_int),
+        "ecnf_qk_norm_rotary_grad": ([P, P, SZ, P], ctypes.c_int),
+        "ecnf_cross_attention_workspace_size": ([P, I32, ctypes.POINTER(SZ)], ctypes.c_int),
+        "ecnf_cross_attention": ([P, P, SZ, P], ctypes.c_int),
+        "ecnf_cross_attention_grad": ([P, P, SZ, P], ctypes.c_int),
     }
     for name, (argtypes, restype) in sig.items():
         if path != LIB_PATH and not hasattr(lib, name):

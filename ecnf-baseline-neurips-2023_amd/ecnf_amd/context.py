@@ -1,0 +1,257 @@
+"""Context operators: attention from a molecule's atoms to an encoder's states of another length, with gradients.
+
+  * :func:`qk_norm_rotary` / :func:`qk_norm_rotary_grad`     per-head norm of queries and keys and the rotation by
+    their positions (one to four axes, e.g. chain / residue / atom) in one pass        (ecnf_qk_norm_rotary)
+  * :func:`cross_attention` / :func:`cross_attention_grad`   softmax(scale q k^T) v     (ecnf_cross_attention)
+
+Tensors are [batch, length, heads, head_dim] in float32, bfloat16 or float16, on one device, with any strides (the last
+dimension contiguous, else it is copied first).  The calls run on the tensors' device and torch's current stream of
+it, allocate outputs and workspace from torch's stream-ordered allocator and never synchronise, so they can be captured
+into a graph.  As everywhere in this package gradients are explicit calls: results carry no autograd history.
+Nothing here falls back to the CPU.
+"""
+from __future__ import annotations
+
+import ctypes
+import struct
+from typing import Optional, Sequence, Tuple
+
+import torch
+
+from . import _lib
+
+_DTYPES = {torch.float32: _lib.DTYPE_F32, torch.bfloat16: _lib.DTYPE_BF16, torch.float16: _lib.DTYPE_F16}
+_POSITIONS = {torch.int32: _lib.POS_I32, torch.int64: _lib.POS_I64, torch.float32: _lib.POS_F32}
+# the layouts of _lib.EcnfQkNorm (its two sides first) and _lib.EcnfAttention: packed at once, which costs a tenth of
+# filling a ctypes structure field by field (tests/test_context.py holds them to the compiled library's layout)
+_QK_NORM = struct.Struct("@" + 2 * "6P8q4i" + "9ifd")
+_ATTENTION = struct.Struct("@12P12q9if")
+_NO_SIDE = (0,) * 18
+
+
+def _tensor(x, name: str, like: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """x [batch, length, heads, head_dim] on a device, its last dimension contiguous; dtype and device of `like`."""
+    if not (torch.is_tensor(x) and x.is_cuda):
+        raise ValueError(f"{name} must be a device (cuda) tensor")
+    if x.dim() != 4:
+        raise ValueError(f"{name} must be [batch, length, heads, head_dim], got {tuple(x.shape)}")
+    if like is None:
+        if x.dtype not in _DTYPES:
+            raise ValueError(f"{name} must be float32, bfloat16 or float16, got {x.dtype}")
+    elif x.dtype != like.dtype or x.device != like.device:
+        raise ValueError(f"{name} must have the dtype and device of q ({like.dtype}, {like.device}), got {x.dtype}, "
+                         f"{x.device}")
+    return x if x.stride(3) == 1 else x.contiguous()
+
+
+def _strides(x: torch.Tensor) -> Tuple[int, int, int]:
+    """Strides of the first three dimensions; 0 where there is one element (torch's may be anything there)."""
+    n, s = x.shape, x.stride()
+    return (s[0] if n[0] > 1 else 0, s[1] if n[1] > 1 else 0, s[2] if n[2] > 1 else 0)
+
+
+def _aligned(x: torch.Tensor) -> torch.Tensor:
+    """x with its rows on 16-byte boundaries (a copy if they are not)."""
+    e = x.element_size()
+    a, b, c = _strides(x)
+    return x if (x.data_ptr() | a * e | b * e | c * e) % 16 == 0 else x.contiguous() if not x.is_contiguous() else x.clone()
+
+
+def _same_shape(x: torch.Tensor, like: torch.Tensor, name: str) -> None:
+    if x.shape != like.shape:
+        raise ValueError(f"{name} must have shape {tuple(like.shape)}, got {tuple(x.shape)}")
+
+
+# ------------------------------------------------------------------------------------------------------ norm + rotation
+def _weight(w, x: torch.Tensor, name: str) -> Optional[torch.Tensor]:
+    if w is None:
+        return None
+    if not (torch.is_tensor(w) and w.device == x.device and w.dim() == 1 and w.shape[0] == x.shape[3]
+            and w.dtype in _DTYPES):
+        raise ValueError(f"{name} must be a floating [head_dim = {x.shape[3]}] tensor on {x.device}")
+    return w.float().contiguous()
+
+
+def _positions(p, x: torch.Tensor, n_axes: int, name: str) -> Tuple[torch.Tensor, int, int]:
+    """(positions, batch stride, token stride)"""
+    if not (torch.is_tensor(p) and p.device == x.device and p.dtype in _POSITIONS):
+        raise ValueError(f"{name} must be an int32, int64 or float32 tensor on {x.device}")
+    B, L = x.shape[0], x.shape[1]
+    if tuple(p.shape) not in ((L, n_axes), (B, L, n_axes)):
+        raise ValueError(f"{name} must be [{L}, {n_axes}] or [{B}, {L}, {n_axes}], got {tuple(p.shape)}")
+    if p.stride(-1) != 1 and n_axes > 1:
+        p = p.contiguous()
+    return p, (p.stride(0) if p.dim() == 3 else 0), p.stride(-2)
+
+
+def _norm_call(sides, axes, theta, eps, interleaved, grad: bool):
+    """sides: (x, weight, positions, output gradient or None, name) of q and k; returns (outputs, weight gradients)."""
+    axes = tuple(int(a) for a in axes)
+    if not 1 <= len(axes) <= 4:
+        raise ValueError("axes must name one to four axes")
+    first = sides[0][0]
+    packed, outs, dws, keep = [], [], [], []
+    for x, w, pos, g, name in sides:
+        if x is None:
+            packed += _NO_SIDE
+            outs.append(None)
+            dws.append(None)
+            continue
+        w32 = _weight(w, x, f"{name}_weight")
+        p, pb, pl = _positions(pos, x, len(axes), f"{name}_positions")
+        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        dw = torch.empty(x.shape[3], dtype=torch.float32, device=x.device) if grad and w is not None else None
+        gs = (0, 0, 0) if g is None else _strides(g)
+        packed += (x.data_ptr(), 0 if g is None else g.data_ptr(), out.data_ptr(), 0 if w32 is None else w32.data_ptr(),
+                   0 if dw is None else dw.data_ptr(), p.data_ptr(), *_strides(x), *gs, pb, pl,
+                   x.shape[0], x.shape[1], x.shape[2], _POSITIONS[p.dtype])
+        outs.append(out)
+        dws.append(dw)
+        keep.append((w32, p))
+    args = _QK_NORM.pack(*packed, _DTYPES[first.dtype], first.shape[3], len(axes), *axes, *(0,) * (4 - len(axes)),
+                         bool(interleaved), first.device.index, eps, theta)
+    lib = _lib.load()
+    stream = torch.cuda.current_stream(first.device).cuda_stream
+    if not grad:
+        _lib.check(lib.ecnf_qk_norm_rotary(args, stream))
+        return outs, dws
+    n = ctypes.c_size_t()
+    _lib.check(lib.ecnf_qk_norm_workspace_size(args, ctypes.byref(n)))
+    ws = torch.empty(n.value, dtype=torch.uint8, device=first.device)
+    _lib.check(lib.ecnf_qk_norm_rotary_grad(args, ws.data_ptr(), n.value, stream))
+    for k, (x, w, _, _, _) in enumerate(sides):
+        if dws[k] is not None and w.dtype != torch.float32:
+            dws[k] = dws[k].to(w.dtype)
+    return outs, dws
+
+
+def qk_norm_rotary(q, k=None, *, q_positions, k_positions=None, axes: Sequence[int], q_weight=None, k_weight=None,
+                   theta: float = 10000.0, eps: float = 1e-6, interleaved: bool = False):
+    """(q', k') for q [B, Lq, Hq, D] and k [C, Lk, Hk, D] (or None): each head y = weight * x / sqrt(mean(x^2) + eps),
+    then axis a, ``axes[a]`` dims wide (in order from dim 0), turns its pair j by position[a] * theta^(-2j / axes[a]).
+    Pairs are (j, j + axes[a] / 2) inside the axis, or neighbours with ``interleaved``; dims behind the axes are not
+    turned.  Positions [L, n_axes] or [batch, L, n_axes], whole (int32, int64) or real (float32); their angles are
+    reduced in fp64, so far positions keep their accuracy.  Weights [D], shared by the heads (None: 1).  D is even and
+    at most 128."""
+    q = _tensor(q, "q")
+    if k is not None:
+        k = _tensor(k, "k", q)
+        if k.shape[3] != q.shape[3]:
+            raise ValueError(f"k must have q's head_dim {q.shape[3]}, got {k.shape[3]}")
+    outs, _ = _norm_call(((q, q_weight, q_positions, None, "q"), (k, k_weight, k_positions, None, "k")), axes,
+                         float(theta), float(eps), interleaved, False)
+    return outs[0], outs[1]
+
+
+def qk_norm_rotary_grad(q_grad, k_grad, q, k=None, *, q_positions, k_positions=None, axes: Sequence[int],
+                        q_weight=None, k_weight=None, theta: float = 10000.0, eps: float = 1e-6,
+                        interleaved: bool = False):
+    """(dq, dk, dq_weight, dk_weight) of :func:`qk_norm_rotary` for the gradients of its outputs (None where the
+    operand is).  Weight gradients are summed in fp32 over all rows in a fixed order."""
+    q = _tensor(q, "q")
+    q_grad = _tensor(q_grad, "q_grad", q)
+    _same_shape(q_grad, q, "q_grad")
+    if k is not None:
+        k = _tensor(k, "k", q)
+        if k.shape[3] != q.shape[3]:
+            raise ValueError(f"k must have q's head_dim {q.shape[3]}, got {k.shape[3]}")
+        k_grad = _tensor(k_grad, "k_grad", q)
+        _same_shape(k_grad, k, "k_grad")
+    outs, dws = _norm_call(((q, q_weight, q_positions, q_grad, "q"), (k, k_weight, k_positions, k_grad, "k")), axes,
+                           float(theta), float(eps), interleaved, True)
+    return outs[0], outs[1], dws[0], dws[1]
+
+
+# ------------------------------------------------------------------------------------------------------ cross attention
+def _lengths(x, n: int, like: torch.Tensor, name: str) -> Optional[torch.Tensor]:
+    if x is None:
+        return None
+    if not (torch.is_tensor(x) and x.device == like.device and x.dtype in (torch.int32, torch.int64)
+            and tuple(x.shape) == (n,)):
+        raise ValueError(f"{name} must be an int32 or int64 [{n}] tensor on {like.device}")
+    return x.to(torch.int32).contiguous()
+
+
+def _attention_operands(q, k, v, query_lengths, context_lengths, context_mask, scale):
+    q = _tensor(q, "q")
+    k, v = _tensor(k, "k", q), _tensor(v, "v", q)
+    _same_shape(v, k, "v")
+    B, _, Hq, D = q.shape
+    C, Lk, Hk = k.shape[:3]
+    if C != B and C != 1:
+        raise ValueError(f"k must have q's batch {B} or 1, got {C}")
+    if k.shape[3] != D:
+        raise ValueError(f"k must have q's head_dim {D}, got {k.shape[3]}")
+    if Hk < 1 or Hq < 1 or Hq % Hk:
+        raise ValueError(f"q's heads ({Hq}) must be a multiple of k's ({Hk})")
+    q, k, v = _aligned(q), _aligned(k), _aligned(v)
+    ql = _lengths(query_lengths, B, q, "query_lengths")
+    cl = _lengths(context_lengths, C, q, "context_lengths")
+    m = context_mask
+    if m is not None:
+        if not (torch.is_tensor(m) and m.device == q.device and m.dtype in (torch.bool, torch.uint8)
+                and tuple(m.shape) == (C, Lk)):
+            raise ValueError(f"context_mask must be a bool [{C}, {Lk}] tensor on {q.device}")
+        m = m.contiguous()
+    return q, k, v, ql, cl, m, float(D ** -0.5 if scale is None else scale)
+
+
+def _attention_args(q, k, v, out, dout, lse, dq, dk, dv, ql, cl, m, scale) -> bytes:
+    B, Lq, Hq, D = q.shape
+    C, Lk, Hk = k.shape[:3]
+
+    def ptr(t):
+        return 0 if t is None else t.data_ptr()
+    return _ATTENTION.pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), ptr(dout), ptr(lse), ptr(dq), ptr(dk),
+                           ptr(dv), ptr(ql), ptr(cl), ptr(m), *_strides(q), *_strides(k), *_strides(v),
+                           *((0, 0, 0) if dout is None else _strides(dout)), _DTYPES[q.dtype], B, C, Lq, Lk, Hq, Hk, D,
+                           q.device.index, scale)
+
+
+def _run_attention(args: bytes, grad: int, device) -> None:
+    lib = _lib.load()
+    n = ctypes.c_size_t()
+    _lib.check(lib.ecnf_cross_attention_workspace_size(args, grad, ctypes.byref(n)))
+    ws = torch.empty(n.value, dtype=torch.uint8, device=device) if n.value else None
+    fn = lib.ecnf_cross_attention_grad if grad else lib.ecnf_cross_attention
+    _lib.check(fn(args, None if ws is None else ws.data_ptr(), n.value, torch.cuda.current_stream(device).cuda_stream))
+
+
+def cross_attention(q, k, v, *, query_lengths=None, context_lengths=None, context_mask=None,
+                    scale: Optional[float] = None, return_lse: bool = False):
+    """softmax(scale q k^T) v for q [B, Lq, Hq, D] and k, v [C, Lk, Hk, D]: out [B, Lq, Hq, D], and with ``return_lse``
+    the rows' log sum exp [B, Hq, Lq] (fp32), which :func:`cross_attention_grad` takes.
+
+    C is B, or 1: one context for the whole batch.  Hq is a multiple of Hk: query head h reads key head
+    h // (Hq // Hk).  D is a multiple of 8, at most 128; scale defaults to D^-0.5.  A row reads the keys below
+    ``context_lengths`` [C] (clamped to [0, Lk]) where ``context_mask`` [C, Lk] is true; what lies behind is never used,
+    NaN included.  A row without keys, and a query at or behind ``query_lengths`` [B], gives 0 and lse -inf."""
+    q, k, v, ql, cl, m, scale = _attention_operands(q, k, v, query_lengths, context_lengths, context_mask, scale)
+    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    lse = torch.empty((q.shape[0], q.shape[2], q.shape[1]), dtype=torch.float32, device=q.device) if return_lse else None
+    if q.shape[0]:
+        _run_attention(_attention_args(q, k, v, out, None, lse, None, None, None, ql, cl, m, scale), 0, q.device)
+    return (out, lse) if return_lse else out
+
+
+def cross_attention_grad(out_grad, q, k, v, out, lse, *, query_lengths=None, context_lengths=None, context_mask=None,
+                         scale: Optional[float] = None):
+    """(dq, dk, dv) of :func:`cross_attention` for ``out_grad``, from its results ``out`` and ``lse``.  The gradients of
+    key heads that several query heads share, and of a context that the whole batch shares, are summed (fp32, in a
+    fixed order); those of keys that no row may read are 0."""
+    q, k, v, ql, cl, m, scale = _attention_operands(q, k, v, query_lengths, context_lengths, context_mask, scale)
+    out_grad, out = _tensor(out_grad, "out_grad", q), _tensor(out, "out", q)
+    _same_shape(out_grad, q, "out_grad")
+    _same_shape(out, q, "out")
+    want = (q.shape[0], q.shape[2], q.shape[1])
+    if not (torch.is_tensor(lse) and lse.device == q.device and lse.dtype == torch.float32 and tuple(lse.shape) == want):
+        raise ValueError(f"lse must be the float32 {want} tensor of cross_attention(return_lse=True)")
+    out_grad, out, lse = _aligned(out_grad), _aligned(out.contiguous()), lse.contiguous()
+    dq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    dk, dv = torch.empty(k.shape, dtype=k.dtype, device=k.device), torch.empty(k.shape, dtype=k.dtype, device=k.device)
+    if q.shape[0]:
+        _run_attention(_attention_args(q, k, v, out, out_grad, lse, dq, dk, dv, ql, cl, m, scale), 1, q.device)
+    else:
+        dk.zero_()
+        dv.zero_()
+    return dq, dk, dv

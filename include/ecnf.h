@@ -265,8 +265,73 @@ int ecnf_adam_update(ecnf_trainer* tr, const float* grad, float* params, float* 
 /* Replace a handle's weights with the blob `params` (on_device: a DEVICE pointer, else host).  Synchronous. */
 int ecnf_update_params(ecnf_handle* h, const float* params, int32_t on_device);
 
+/* ---- context operators (no handle needed): attention from the atoms to an encoder's states of another length ----
+ * The reference's field knows its molecule by an embedded id per atom only; these operators make a node embedding that
+ * also reads a context (ecnf_amd.context; ecnf_integrate_nodes and its kin take it).
+ *   - tensors are [batch, length, heads, head_dim] in any of ecnf_dtype; strides in elements for the first three
+ *     dimensions, the last one contiguous; outputs and gradients are contiguous.
+ *   - `device` is the operands' device: it is made current for the launches and the caller's restored.
+ *   - sums, softmax statistics and norms are fp32 (the rotation's angles fp64); no sum's order depends on the launch.
+ *   - a call may be captured into a graph; the workspace is the caller's and belongs to the call until it has run. */
+enum ecnf_dtype { ECNF_DTYPE_F32 = 0, ECNF_DTYPE_BF16 = 1, ECNF_DTYPE_F16 = 2 };
+enum ecnf_position_type { ECNF_POS_I32 = 0, ECNF_POS_I64 = 1, ECNF_POS_F32 = 2 };
+
+/* One of the two tensors of ecnf_qk_norm (q or k); length 0: absent. */
+typedef struct ecnf_qk_side {
+  const void* x;              /* [batch, length, heads, head_dim]                                     */
+  const void* grad;           /* backward: the gradient of the output                                 */
+  void* out;                  /* forward: the output; backward: the gradient of x (contiguous)        */
+  const float* weight;        /* [head_dim], shared by the heads; NULL: 1                             */
+  float* weight_grad;         /* backward, with a weight: [head_dim]                                  */
+  const void* positions;      /* [batch, length, n_axes], last dimension contiguous                   */
+  int64_t x_stride[3], grad_stride[3];
+  int64_t position_stride[2]; /* batch (0: the same for every molecule), token                        */
+  int32_t batch, length, heads;
+  int32_t position_type;      /* ecnf_position_type                                                   */
+} ecnf_qk_side;
+
+/* y = weight * x / sqrt(mean(x^2) + eps) for each head, then for axis a of axes[a] dims (in order from dim 0) pair j
+ * turned by position[a] * theta^(-2j / axes[a]): pairs are (j, j + axes[a] / 2) inside the axis, or neighbours when
+ * interleaved; dims behind the axes are not turned. */
+typedef struct ecnf_qk_norm {
+  ecnf_qk_side q, k;
+  int32_t dtype, head_dim, n_axes; /* head_dim: even, <= 128; 1 to 4 axes */
+  int32_t axes[4];
+  int32_t interleaved, device;
+  float eps;
+  double theta;
+} ecnf_qk_norm;
+int ecnf_qk_norm_rotary(const ecnf_qk_norm* o, void* stream);
+int ecnf_qk_norm_workspace_size(const ecnf_qk_norm* o, size_t* bytes); /* of the backward pass */
+int ecnf_qk_norm_rotary_grad(const ecnf_qk_norm* o, void* workspace, size_t workspace_bytes, void* stream);
+
+/* out = softmax(scale q k^T) v over each row's allowed keys (key < context_lengths[c] and context_mask[c][key] != 0).
+ * A row without keys, and a query at or behind query_lengths[b], gives 0 (lse -inf) and no gradient; what memory holds
+ * behind a mask or a length is not used.  heads is a multiple of kv_heads (query head h reads key head
+ * h / (heads / kv_heads)); context_batch is batch, or 1: one context for the whole batch (its gradients are summed over
+ * the batch).  Rows of every operand start on 16-byte boundaries. */
+typedef struct ecnf_attention {
+  const void *q, *k, *v;      /* [batch, n_queries, heads, head_dim], [context_batch, context_length, kv_heads, ..] */
+  void* out;                  /* forward: written; backward: the forward's output                                  */
+  const void* out_grad;       /* backward                                                                          */
+  float* lse;                 /* [batch, heads, n_queries] log sum exp; forward: written unless NULL; backward: read */
+  void *q_grad, *k_grad, *v_grad;
+  const int32_t* query_lengths;   /* [batch] or NULL                       */
+  const int32_t* context_lengths; /* [context_batch] or NULL               */
+  const uint8_t* context_mask;    /* [context_batch, context_length] or NULL */
+  int64_t q_stride[3], k_stride[3], v_stride[3], out_grad_stride[3];
+  int32_t dtype, batch, context_batch, n_queries, context_length, heads, kv_heads;
+  int32_t head_dim;           /* a multiple of 8 in [8, 128] */
+  int32_t device;
+  float scale;
+} ecnf_attention;
+int ecnf_cross_attention_workspace_size(const ecnf_attention* o, int32_t grad, size_t* bytes);
+int ecnf_cross_attention(const ecnf_attention* o, void* workspace, size_t workspace_bytes, void* stream);
+int ecnf_cross_attention_grad(const ecnf_attention* o, void* workspace, size_t workspace_bytes, void* stream);
+
 /* Layout of the ABI structs as this library was compiled: out[0] = sizeof, out[1 + i] = offsetof field i (declaration
- * order) for which = 0 ecnf_cfg, 1 ecnf_solve_opts, 2 ecnf_target, 3 ecnf_adam_opts.  Writes min(cap, 1 + fields)
+ * order) for which = 0 ecnf_cfg, 1 ecnf_solve_opts, 2 ecnf_target, 3 ecnf_adam_opts, 4 ecnf_qk_side, 5 ecnf_qk_norm,
+ * 6 ecnf_attention.  Writes min(cap, 1 + fields)
  * values and returns the number of fields (-1 for an unknown `which`).  Bindings (ctypes, cgo, ...) check their struct
  * mirrors against it. */
 int ecnf_struct_layout(int32_t which, size_t* out, int32_t cap);
