@@ -696,10 +696,32 @@ bool tail_teams(const ecnf_handle* h, int NT, int div, int mpw) {
          team_shape(c.mlp_width, 1, c.mlp_depth, c.dim, 0);
 }
 
+// A call's own embedding table (ecnf_integrate_nodes and its kin): the kernels read its rows where they read the
+// handle's nn.Embed rows.  Atoms of one molecule may then enter block 1 with different rows, so the block-1 pair tiles
+// (equal rows) are off.  Index arithmetic in the kernels is 32-bit: rows * hidden < 2^31.
+struct NodeTable {
+  const float* emb = nullptr;
+  int32_t rows = 0;
+  void apply(Net* net) const {
+    if (!emb) return;
+    net->emb = emb;
+    net->nfeat = rows;
+    net->pairs = 0;
+  }
+};
+
+int check_nodes(const ecnf_cfg& c, const float* nodes, int32_t n_rows) {
+  if (!nodes) return fail(ECNF_E_INVALID, "NULL argument");
+  if (n_rows < 1) return fail(ECNF_E_INVALID, "n_rows must be >= 1");
+  if ((int64_t)n_rows * c.hidden >= (1ll << 31)) return fail(ECNF_E_UNSUPPORTED, "n_rows * hidden must stay below 2^31");
+  return ECNF_OK;
+}
+
 // G, cols: team_size's decision for this solve (G = 1: the batch path)
 hipError_t dispatch_integrate(const ecnf_handle* h, int NT, const SolveP& sp_in, int G, int cols, const float* y0,
                               const int32_t* feat, const float* eps, float* y1, float* dlogp, int32_t* nfe,
-                              int32_t* status, int B, hipStream_t stream, float* sched = nullptr) {
+                              int32_t* status, int B, hipStream_t stream, const NodeTable& nodes,
+                              float* sched = nullptr) {
   const int M = h->cfg.mlp_width, L = h->cfg.mlp_depth, D = h->cfg.dim, P = h->prec, ix = 2 * P + NT;
   size_t lds = 0;
   SolveP sp = sp_in;
@@ -727,6 +749,7 @@ hipError_t dispatch_integrate(const ecnf_handle* h, int NT, const SolveP& sp_in,
     sp.team = TeamP{};
     net = net_for_batch(h, ix, B, &lds, sp.adaptive != 0);
   }
+  nodes.apply(&net);
   auto launch = [&](const SolveP& spl) -> hipError_t {
 #define ECNF_CALL(m, l, d, nt, p) \
   launch_integrate<m / 32, nt, l, d, p>(net, lds, spl, y0, feat, eps, y1, dlogp, nfe, status, B, stream)
@@ -817,10 +840,12 @@ hipError_t dispatch_integrate(const ecnf_handle* h, int NT, const SolveP& sp_in,
 }
 
 hipError_t dispatch_vf(const ecnf_handle* h, int NT, const float* x, const float* t, const int32_t* feat,
-                       const float* tan_in, int ntan, float* v, float* tan_out, int B, hipStream_t stream) {
+                       const float* tan_in, int ntan, float* v, float* tan_out, int B, hipStream_t stream,
+                       const NodeTable& nodes = {}) {
   const int M = h->cfg.mlp_width, L = h->cfg.mlp_depth, D = h->cfg.dim, P = h->prec, ix = 2 * P + NT;
   size_t lds = 0;
-  const Net net = net_for_batch(h, ix, B, &lds);
+  Net net = net_for_batch(h, ix, B, &lds);
+  nodes.apply(&net);
 #define ECNF_CALL(m, l, d, nt, p) \
   launch_vf<m / 32, nt, l, d, p>(net, lds, x, t, feat, tan_in, ntan, v, tan_out, B, stream)
 #define X(m, l, d)                                                                                           \
@@ -887,7 +912,7 @@ size_t sched_floats(const ecnf_handle* h, const ecnf_solve_opts* o, int batch) {
 
 int integrate_impl(ecnf_handle* h, const ecnf_solve_opts* o, const float* y0, const int32_t* feat, const float* eps,
                    float* y1, float* dlogp, int32_t* nfe, int32_t* status, int32_t batch, float* ws, size_t ws_bytes,
-                   hipStream_t stream, bool arena);
+                   hipStream_t stream, bool arena, const NodeTable& nodes = {});
 
 }  // namespace
 
@@ -1378,6 +1403,19 @@ int ecnf_vector_field(ecnf_handle* h, const float* x, const float* t, const int3
   return ECNF_OK;
 }
 
+int ecnf_vector_field_nodes(ecnf_handle* h, const float* x, const float* t, const float* nodes, int32_t n_rows,
+                            const int32_t* row, float* v, int32_t batch, void* stream) {
+  if (!h) return fail(ECNF_E_INVALID, "NULL handle");
+  if (batch < 0) return fail(ECNF_E_INVALID, "batch < 0");
+  if (batch == 0) return ECNF_OK;
+  if (!x || !t || !row || !v) return fail(ECNF_E_INVALID, "NULL argument");
+  if (int rc = check_nodes(h->cfg, nodes, n_rows)) return rc;
+  HIP_TRY(hipSetDevice(h->device));
+  HIP_TRY(dispatch_vf(h, 0, x, t, row, nullptr, 0, v, nullptr, batch, (hipStream_t)stream, NodeTable{nodes, n_rows}));
+  g_err.clear();
+  return ECNF_OK;
+}
+
 int ecnf_vf_jvp(ecnf_handle* h, const float* x, const float* t, const int32_t* feat, const float* tan_in,
                 int32_t n_tangents, float* v, float* tan_out, int32_t batch, void* stream) {
   if (!h) return fail(ECNF_E_INVALID, "NULL handle");
@@ -1471,6 +1509,20 @@ int ecnf_integrate_ws(ecnf_handle* h, const ecnf_solve_opts* o, const float* y0,
                         (hipStream_t)stream, false);
 }
 
+int ecnf_integrate_nodes(ecnf_handle* h, const ecnf_solve_opts* o, const float* y0, const float* nodes, int32_t n_rows,
+                         const int32_t* row, const float* eps, float* y1, float* dlogp, int32_t* nfe, int32_t* status,
+                         int32_t batch, void* workspace, size_t workspace_bytes, void* stream) {
+  if (!h || !o) return fail(ECNF_E_INVALID, "NULL handle/options");
+  if (batch < 0) return fail(ECNF_E_INVALID, "batch < 0");
+  if (batch > 0)
+    if (int rc = check_nodes(h->cfg, nodes, n_rows)) return rc;
+  if (workspace && batch > 0 && exact_sparse(h, o->divergence) &&
+      workspace_bytes < pcache_floats(h, batch) * sizeof(float))
+    return fail(ECNF_E_INVALID, "workspace smaller than ecnf_integrate_workspace_size");
+  return integrate_impl(h, o, y0, row, eps, y1, dlogp, nfe, status, batch, (float*)workspace, workspace_bytes,
+                        (hipStream_t)stream, false, NodeTable{nodes, n_rows});
+}
+
 int ecnf_integrate(ecnf_handle* h, const ecnf_solve_opts* o, const float* y0, const int32_t* feat, const float* eps,
                    float* y1, float* dlogp, int32_t* nfe, int32_t* status, int32_t batch, void* stream) {
   if (!h || !o) return fail(ECNF_E_INVALID, "NULL handle/options");
@@ -1486,7 +1538,7 @@ namespace {
 
 int integrate_impl(ecnf_handle* h, const ecnf_solve_opts* o, const float* y0, const int32_t* feat, const float* eps,
                    float* y1, float* dlogp, int32_t* nfe, int32_t* status, int32_t batch, float* ws, size_t ws_bytes,
-                   hipStream_t stream, bool arena) {
+                   hipStream_t stream, bool arena, const NodeTable& nodes) {
   if (batch > 0 && (!y0 || !feat || !y1)) return fail(ECNF_E_INVALID, "NULL argument");
   if (o->solver != ECNF_SOLVER_EULER && o->solver != ECNF_SOLVER_DOPRI5) return fail(ECNF_E_INVALID, "unknown solver");
   if (o->divergence < ECNF_DIV_NONE || o->divergence > ECNF_DIV_EXACT) return fail(ECNF_E_INVALID, "unknown divergence");
@@ -1570,7 +1622,7 @@ int integrate_impl(ecnf_handle* h, const ecnf_solve_opts* o, const float* y0, co
     // (arena_mu, held since the arena was read)
     if (!h->arena_ev) HIP_TRY(hipEventCreateWithFlags(&h->arena_ev, hipEventDisableTiming));
     if (h->arena_used && h->arena_stream != stream) HIP_TRY(hipStreamWaitEvent(stream, h->arena_ev, 0));
-    HIP_TRY(dispatch_integrate(h, NT, sp, G, cols, y0, feat, eps, y1, dlogp, nfe, status, batch, stream, sched));
+    HIP_TRY(dispatch_integrate(h, NT, sp, G, cols, y0, feat, eps, y1, dlogp, nfe, status, batch, stream, nodes, sched));
     HIP_TRY(team_done());
     HIP_TRY(hipEventRecord(h->arena_ev, stream));
     h->arena_used = true;
@@ -1580,12 +1632,12 @@ int integrate_impl(ecnf_handle* h, const ecnf_solve_opts* o, const float* y0, co
     std::lock_guard<std::mutex> tl(h->team_mu);
     if (!h->team_ev) HIP_TRY(hipEventCreateWithFlags(&h->team_ev, hipEventDisableTiming));
     if (h->team_used && h->team_stream != stream) HIP_TRY(hipStreamWaitEvent(stream, h->team_ev, 0));
-    HIP_TRY(dispatch_integrate(h, NT, sp, G, cols, y0, feat, eps, y1, dlogp, nfe, status, batch, stream));
+    HIP_TRY(dispatch_integrate(h, NT, sp, G, cols, y0, feat, eps, y1, dlogp, nfe, status, batch, stream, nodes));
     HIP_TRY(hipEventRecord(h->team_ev, stream));
     h->team_used = true;
     h->team_stream = stream;
   } else {
-    HIP_TRY(dispatch_integrate(h, NT, sp, G, cols, y0, feat, eps, y1, dlogp, nfe, status, batch, stream, sched));
+    HIP_TRY(dispatch_integrate(h, NT, sp, G, cols, y0, feat, eps, y1, dlogp, nfe, status, batch, stream, nodes, sched));
     HIP_TRY(team_done());
   }
   g_err.clear();

@@ -881,106 +881,14 @@ struct Launcher {
 
 }  // namespace
 
-extern "C" {
-
-int ecnf_trainer_create(const ecnf_cfg* cfg, int32_t max_batch, int device, ecnf_trainer** out) {
-  size_t n = 0;
-  int rc = ecnf_param_count(cfg, &n);   // validates the config
-  if (rc) return rc;
-  if (!out) return fail(ECNF_E_INVALID, "out is NULL");
-  if (max_batch < 1) return fail(ECNF_E_INVALID, "max_batch must be >= 1");
-  if (cfg->n_nodes * cfg->dim > kMaxND) return fail(ECNF_E_UNSUPPORTED, "training needs n_nodes * dim <= 256");
-  const ecnf_cfg c = *cfg;
-  const long B = max_batch, N = c.n_nodes, D = c.dim, H = c.hidden, T = c.time_embedding_dim, M = c.mlp_width,
-             L = c.mlp_depth, K = c.n_blocks;
-  const long E = N * (N - 1), BN = B * N, BE = B * E;
-  ecnf_trainer* tr = new ecnf_trainer();
-  tr->cfg = c;
-  tr->device = device;
-  tr->max_batch = max_batch;
-  tr->off = param_offsets(c);
-  const int half = (int)T / 2;
-  const float ex = std::log(10000.0f) / (float)(half - 1);
-  for (int k = 0; k < 8; ++k) tr->freqs[k] = k < half ? std::exp((float)k * -ex) : 0.f;
-  // arena layout
-  std::vector<std::pair<float**, long>> plan;
-  auto add = [&](float** p, long nf) { plan.push_back({p, (nf + 63) & ~63L}); };
-  add(&tr->ut, B * N * D); add(&tr->mean, B * D); add(&tr->temb, B * T);
-  add(&tr->part_loss, B); add(&tr->part_dfs, B); add(&tr->dxa, BN * D); add(&tr->dxb, BN * D);
-  add(&tr->norm_part, 2 * ((n + 255) / 256) + 64);
-  tr->xc.resize(K + 1); tr->hin.resize(K); tr->h1.resize(K); tr->Ps.resize(K); tr->Pr.resize(K); tr->r.resize(K);
-  tr->len.resize(K); tr->px.resize(K); tr->gate.resize(K); tr->hcat.resize(K);
-  tr->ze.resize(K * L); tr->ae.resize(K * L); tr->zx.resize(K * L); tr->ax.resize(K * L);
-  tr->zh.resize(K * (L + 1)); tr->ah.resize(K * (L + 1));
-  for (long k = 0; k <= K; ++k) add(&tr->xc[k], BN * D);
-  for (long k = 0; k < K; ++k) {
-    add(&tr->hin[k], BN * (H + T)); add(&tr->h1[k], BN * H); add(&tr->Ps[k], BN * M); add(&tr->Pr[k], BN * M);
-    add(&tr->r[k], BE * D); add(&tr->len[k], BE); add(&tr->px[k], BE); add(&tr->gate[k], BE);
-    add(&tr->hcat[k], BN * (M + H));
-    for (long l = 0; l < L; ++l) {
-      add(&tr->ze[k * L + l], BE * M); add(&tr->ae[k * L + l], BE * M);
-      add(&tr->zx[k * L + l], BE * M); add(&tr->ax[k * L + l], BE * M);
-    }
-    for (long l = 0; l <= L; ++l) {
-      add(&tr->zh[k * (L + 1) + l], BN * std::max(M, H)); add(&tr->ah[k * (L + 1) + l], BN * M);
-    }
-  }
-  add(&tr->dA, BE * M); add(&tr->dB, BE * M); add(&tr->dm_gate, BE * M); add(&tr->de, BE); add(&tr->dpx, BE);
-  add(&tr->dr, BE * D); add(&tr->dPs, BN * M); add(&tr->dPr, BN * M); add(&tr->dhcat, BN * (M + H));
-  add(&tr->dh1, BN * H); add(&tr->dhin, BN * (H + T)); add(&tr->dhA, BN * M); add(&tr->dhB, BN * M);
-  add(&tr->dhn, BN * H);
-  // partial arena of the deferred split reductions: at least 128 splits of the largest weight block and its bias
-  // ((M + H) x M, (H + T) x H) and the embedding gradient's row-chunk partials; 32 M floats (128 MiB) when larger,
-  // which holds a whole LJ13 step's partials in about two flushes
-  tr->red_floats = (size_t)std::max<long>({128 * (std::max((M + H) * M, (H + T) * H) + std::max(M + H, H + T) + 256),
-                                           ((BN + 63) / 64) * (long)c.n_features * H + 64, 32L << 20});
-  add(&tr->red, (long)tr->red_floats);
-  tr->red_capacity = tr->red_floats;
-  tr->red_min = (size_t)(((BN + 63) / 64) * (long)c.n_features * H + 64);
-  size_t total = 0;
-  for (auto& q : plan) total += (size_t)q.second;
-  tr->arena_floats = total;
-  int ndev = 0;
-  hipError_t e = hipGetDeviceCount(&ndev);
-  if (e != hipSuccess || device < 0 || device >= ndev) {
-    delete tr;
-    return e != hipSuccess ? fail(ECNF_E_HIP, std::string("hipGetDeviceCount: ") + hipGetErrorString(e))
-                           : fail(ECNF_E_INVALID, "device index out of range");
-  }
-  if ((e = hipSetDevice(device)) != hipSuccess || (e = hipMalloc(&tr->arena, total * sizeof(float))) != hipSuccess) {
-    delete tr;
-    return fail(ECNF_E_HIP, std::string("trainer allocation: ") + hipGetErrorString(e));
-  }
-  float* p = tr->arena;
-  for (auto& q : plan) {
-    *q.first = p;
-    p += q.second;
-  }
-  *out = tr;
-  return ECNF_OK;
-}
-
-int ecnf_trainer_destroy(ecnf_trainer* tr) {
-  if (!tr) return ECNF_OK;
-  TR_TRY(hipSetDevice(tr->device));
-  TR_TRY(hipDeviceSynchronize());
-  TR_TRY(hipFree(tr->arena));
-  delete tr;
-  return ECNF_OK;
-}
-
-int ecnf_trainer_set_reduction_arena(ecnf_trainer* tr, size_t floats, size_t* used) {
-  if (!tr) return fail(ECNF_E_INVALID, "NULL trainer");
-  tr->red_floats = floats == 0 ? tr->red_capacity : std::min(tr->red_capacity, std::max(tr->red_min, floats));
-  if (used) *used = tr->red_floats;
-  return ECNF_OK;
-}
-
-int ecnf_fm_loss_grad(ecnf_trainer* tr, const float* params, const float* x1, const float* x0, const float* t,
-                      const int32_t* feat, float sigma_min, int32_t batch, float* loss, float* grad, void* stream) {
+// the training step of ecnf_fm_loss_grad (feat: embedding ids) and ecnf_fm_loss_grad_nodes (nodes [batch, N, H]: the
+// rows themselves; their gradient goes to nodes_grad and the table's is 0)
+static int loss_grad(ecnf_trainer* tr, const float* params, const float* x1, const float* x0, const float* t,
+                     const int32_t* feat, const float* nodes, float* nodes_grad, float sigma_min, int32_t batch,
+                     float* loss, float* grad, void* stream) {
   if (!tr) return fail(ECNF_E_INVALID, "NULL trainer");
   if (batch < 1 || batch > tr->max_batch) return fail(ECNF_E_INVALID, "batch must be in [1, max_batch]");
-  if (!params || !x1 || !x0 || !t || !feat || !loss || !grad) return fail(ECNF_E_INVALID, "NULL argument");
+  if (!params || !x1 || !x0 || !t || !loss || !grad) return fail(ECNF_E_INVALID, "NULL argument");
   const ecnf_cfg& c = tr->cfg;
   Geom G{batch, c.n_nodes, c.dim, c.hidden, c.time_embedding_dim, c.mlp_width, c.mlp_depth, c.n_blocks,
          c.n_nodes * (c.n_nodes - 1), c.n_features, c.normalization_constant, sigma_min};
@@ -1005,8 +913,8 @@ int ecnf_fm_loss_grad(ecnf_trainer* tr, const float* params, const float* x1, co
     const BlockOff& bo = o.blk[k];
     // hin = [h | temb]; h1 = hin Wn + bn  (egnn.py:166-167)
     if (k == 0)
-      hipLaunchKernelGGL(k_hin, dim3(nb(BN * (H + T))), dim3(256), 0, s, G, (const float*)nullptr, 0L, feat,
-                         P + o.emb, (const float*)tr->temb, tr->hin[0]);
+      hipLaunchKernelGGL(k_hin, dim3(nb(BN * (H + T))), dim3(256), 0, s, G, nodes, H, feat, P + o.emb,
+                         (const float*)tr->temb, tr->hin[0]);
     else
       hipLaunchKernelGGL(k_hin, dim3(nb(BN * (H + T))), dim3(256), 0, s, G, (const float*)tr->zh[(k - 1) * (L + 1) + L],
                          H, (const int32_t*)nullptr, (const float*)nullptr, (const float*)tr->temb, tr->hin[k]);
@@ -1160,7 +1068,11 @@ int ecnf_fm_loss_grad(ecnf_trainer* tr, const float* params, const float* x1, co
       dh_next = tr->dhn;
     }
   }
-  {
+  if (nodes) {   // d loss / d nodes = dhin[:, :H]
+    hipLaunchKernelGGL(k_copy_add, dim3(nb(BN * H)), dim3(256), 0, s, BN, (int)H, (const float*)tr->dhin, H + T,
+                       (const float*)nullptr, 0L, nodes_grad, H);
+    Lc.check();
+  } else {
     const unsigned chunks = (unsigned)((BN + 63) / 64), hc = (unsigned)((H + 63) / 64);
     const long ne = (long)G.nfeat * H;
     float* part = Lc.red_alloc((size_t)chunks * ne);
@@ -1172,6 +1084,114 @@ int ecnf_fm_loss_grad(ecnf_trainer* tr, const float* params, const float* x1, co
   Lc.flush();
   if (Lc.err != hipSuccess) return fail(ECNF_E_HIP, std::string("training step launch: ") + hipGetErrorString(Lc.err));
   return ECNF_OK;
+}
+
+extern "C" {
+
+int ecnf_trainer_create(const ecnf_cfg* cfg, int32_t max_batch, int device, ecnf_trainer** out) {
+  size_t n = 0;
+  int rc = ecnf_param_count(cfg, &n);   // validates the config
+  if (rc) return rc;
+  if (!out) return fail(ECNF_E_INVALID, "out is NULL");
+  if (max_batch < 1) return fail(ECNF_E_INVALID, "max_batch must be >= 1");
+  if (cfg->n_nodes * cfg->dim > kMaxND) return fail(ECNF_E_UNSUPPORTED, "training needs n_nodes * dim <= 256");
+  const ecnf_cfg c = *cfg;
+  const long B = max_batch, N = c.n_nodes, D = c.dim, H = c.hidden, T = c.time_embedding_dim, M = c.mlp_width,
+             L = c.mlp_depth, K = c.n_blocks;
+  const long E = N * (N - 1), BN = B * N, BE = B * E;
+  ecnf_trainer* tr = new ecnf_trainer();
+  tr->cfg = c;
+  tr->device = device;
+  tr->max_batch = max_batch;
+  tr->off = param_offsets(c);
+  const int half = (int)T / 2;
+  const float ex = std::log(10000.0f) / (float)(half - 1);
+  for (int k = 0; k < 8; ++k) tr->freqs[k] = k < half ? std::exp((float)k * -ex) : 0.f;
+  // arena layout
+  std::vector<std::pair<float**, long>> plan;
+  auto add = [&](float** p, long nf) { plan.push_back({p, (nf + 63) & ~63L}); };
+  add(&tr->ut, B * N * D); add(&tr->mean, B * D); add(&tr->temb, B * T);
+  add(&tr->part_loss, B); add(&tr->part_dfs, B); add(&tr->dxa, BN * D); add(&tr->dxb, BN * D);
+  add(&tr->norm_part, 2 * ((n + 255) / 256) + 64);
+  tr->xc.resize(K + 1); tr->hin.resize(K); tr->h1.resize(K); tr->Ps.resize(K); tr->Pr.resize(K); tr->r.resize(K);
+  tr->len.resize(K); tr->px.resize(K); tr->gate.resize(K); tr->hcat.resize(K);
+  tr->ze.resize(K * L); tr->ae.resize(K * L); tr->zx.resize(K * L); tr->ax.resize(K * L);
+  tr->zh.resize(K * (L + 1)); tr->ah.resize(K * (L + 1));
+  for (long k = 0; k <= K; ++k) add(&tr->xc[k], BN * D);
+  for (long k = 0; k < K; ++k) {
+    add(&tr->hin[k], BN * (H + T)); add(&tr->h1[k], BN * H); add(&tr->Ps[k], BN * M); add(&tr->Pr[k], BN * M);
+    add(&tr->r[k], BE * D); add(&tr->len[k], BE); add(&tr->px[k], BE); add(&tr->gate[k], BE);
+    add(&tr->hcat[k], BN * (M + H));
+    for (long l = 0; l < L; ++l) {
+      add(&tr->ze[k * L + l], BE * M); add(&tr->ae[k * L + l], BE * M);
+      add(&tr->zx[k * L + l], BE * M); add(&tr->ax[k * L + l], BE * M);
+    }
+    for (long l = 0; l <= L; ++l) {
+      add(&tr->zh[k * (L + 1) + l], BN * std::max(M, H)); add(&tr->ah[k * (L + 1) + l], BN * M);
+    }
+  }
+  add(&tr->dA, BE * M); add(&tr->dB, BE * M); add(&tr->dm_gate, BE * M); add(&tr->de, BE); add(&tr->dpx, BE);
+  add(&tr->dr, BE * D); add(&tr->dPs, BN * M); add(&tr->dPr, BN * M); add(&tr->dhcat, BN * (M + H));
+  add(&tr->dh1, BN * H); add(&tr->dhin, BN * (H + T)); add(&tr->dhA, BN * M); add(&tr->dhB, BN * M);
+  add(&tr->dhn, BN * H);
+  // partial arena of the deferred split reductions: at least 128 splits of the largest weight block and its bias
+  // ((M + H) x M, (H + T) x H) and the embedding gradient's row-chunk partials; 32 M floats (128 MiB) when larger,
+  // which holds a whole LJ13 step's partials in about two flushes
+  tr->red_floats = (size_t)std::max<long>({128 * (std::max((M + H) * M, (H + T) * H) + std::max(M + H, H + T) + 256),
+                                           ((BN + 63) / 64) * (long)c.n_features * H + 64, 32L << 20});
+  add(&tr->red, (long)tr->red_floats);
+  tr->red_capacity = tr->red_floats;
+  tr->red_min = (size_t)(((BN + 63) / 64) * (long)c.n_features * H + 64);
+  size_t total = 0;
+  for (auto& q : plan) total += (size_t)q.second;
+  tr->arena_floats = total;
+  int ndev = 0;
+  hipError_t e = hipGetDeviceCount(&ndev);
+  if (e != hipSuccess || device < 0 || device >= ndev) {
+    delete tr;
+    return e != hipSuccess ? fail(ECNF_E_HIP, std::string("hipGetDeviceCount: ") + hipGetErrorString(e))
+                           : fail(ECNF_E_INVALID, "device index out of range");
+  }
+  if ((e = hipSetDevice(device)) != hipSuccess || (e = hipMalloc(&tr->arena, total * sizeof(float))) != hipSuccess) {
+    delete tr;
+    return fail(ECNF_E_HIP, std::string("trainer allocation: ") + hipGetErrorString(e));
+  }
+  float* p = tr->arena;
+  for (auto& q : plan) {
+    *q.first = p;
+    p += q.second;
+  }
+  *out = tr;
+  return ECNF_OK;
+}
+
+int ecnf_trainer_destroy(ecnf_trainer* tr) {
+  if (!tr) return ECNF_OK;
+  TR_TRY(hipSetDevice(tr->device));
+  TR_TRY(hipDeviceSynchronize());
+  TR_TRY(hipFree(tr->arena));
+  delete tr;
+  return ECNF_OK;
+}
+
+int ecnf_trainer_set_reduction_arena(ecnf_trainer* tr, size_t floats, size_t* used) {
+  if (!tr) return fail(ECNF_E_INVALID, "NULL trainer");
+  tr->red_floats = floats == 0 ? tr->red_capacity : std::min(tr->red_capacity, std::max(tr->red_min, floats));
+  if (used) *used = tr->red_floats;
+  return ECNF_OK;
+}
+
+int ecnf_fm_loss_grad(ecnf_trainer* tr, const float* params, const float* x1, const float* x0, const float* t,
+                      const int32_t* feat, float sigma_min, int32_t batch, float* loss, float* grad, void* stream) {
+  if (!feat) return fail(ECNF_E_INVALID, "NULL argument");
+  return loss_grad(tr, params, x1, x0, t, feat, nullptr, nullptr, sigma_min, batch, loss, grad, stream);
+}
+
+int ecnf_fm_loss_grad_nodes(ecnf_trainer* tr, const float* params, const float* x1, const float* x0, const float* t,
+                            const float* nodes, float sigma_min, int32_t batch, float* loss, float* grad,
+                            float* nodes_grad, void* stream) {
+  if (!nodes || !nodes_grad) return fail(ECNF_E_INVALID, "NULL argument");
+  return loss_grad(tr, params, x1, x0, t, nullptr, nodes, nodes_grad, sigma_min, batch, loss, grad, stream);
 }
 
 int ecnf_adam_update(ecnf_trainer* tr, const float* grad, float* params, float* mu, float* nu, float* ema, size_t n,

@@ -30,6 +30,7 @@ EXPORTED_SYMBOLS = (
     "ecnf_set_team", "ecnf_team_workgroups", "ecnf_integrate_plan",
     "ecnf_qk_norm_rotary", "ecnf_qk_norm_workspace_size", "ecnf_qk_norm_rotary_grad",
     "ecnf_cross_attention_workspace_size", "ecnf_cross_attention", "ecnf_cross_attention_grad",
+    "ecnf_vector_field_nodes", "ecnf_integrate_nodes", "ecnf_fm_loss_grad_nodes",
 )
 
 TARGET_LJ, TARGET_DW = 0, 1
@@ -218,6 +219,10 @@ def load(path: Optional[str] = None) -> ctypes.CDLL:
         "ecnf_integrate_plan": ([P, ctypes.POINTER(EcnfSolveOpts), I32, ctypes.POINTER(I32), ctypes.POINTER(I32)],
                                 ctypes.c_int),
         "ecnf_struct_layout": ([I32, ctypes.POINTER(SZ), I32], ctypes.c_int),
+        "ecnf_vector_field_nodes": ([P, P, P, P, I32, P, P, I32, P], ctypes.c_int),
+        "ecnf_integrate_nodes": ([P, ctypes.POINTER(EcnfSolveOpts), P, P, I32, P, P, P, P, P, P, I32, P, SZ, P],
+                                 ctypes.c_int),
+        "ecnf_fm_loss_grad_nodes": ([P, P, P, P, P, P, ctypes.c_float, I32, P, P, P, P], ctypes.c_int),
         # the context operators' argument structs are passed as packed bytes (ecnf_amd.context)
         "ecnf_qk_norm_rotary": ([P, P], ctypes.c_int),
         "ecnf_qk_norm_workspace_size": ([P, ctypes.POINTER(SZ)], ctypes.c_int),

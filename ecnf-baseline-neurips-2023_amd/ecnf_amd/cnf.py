@@ -101,6 +101,15 @@ def _generator(key, device) -> torch.Generator:
     return g
 
 
+def _node_embedding(h: EcnfHandle, features, context):
+    """None without a context; else the node embeddings that read it (ecnf_amd.context).  They depend on neither x nor
+    t: computed once, whatever the number of evaluations of the solve."""
+    if context is None:
+        return None
+    from .context import node_embedding
+    return node_embedding(h.embedding, features, context, h.cfg)
+
+
 def _batched(features, cfg: CNFConfig, n: Optional[int]):
     """Returns (features [B, N] or None, B, squeeze)."""
     if features is None:
@@ -144,7 +153,7 @@ def build_cnf(n_frames: int, dim: int, sigma_min: float, base_scale: float, n_bl
         # reference-shaped params of a padded config are zero-padded by flatten_params (cfg.ref_mlp_units)
         return device_params(params, cfg, dev)
 
-    def apply(params, x, t, features=None):
+    def apply(params, x, t, features=None, *, context=None):
         h = to_device(params)
         x = torch.as_tensor(x, device=dev, dtype=torch.float32)
         if x.dim() != 2:
@@ -152,7 +161,7 @@ def build_cnf(n_frames: int, dim: int, sigma_min: float, base_scale: float, n_bl
         t = torch.as_tensor(t, device=dev, dtype=torch.float32)
         if t.dim() != 1:
             raise ValueError("time must be rank 1 (build_cnf.py:75)")
-        return h.vector_field(x, t, features)
+        return h.vector_field(x, t, features, node_embedding=_node_embedding(h, features, context))
 
     def sample_base(key, n: int):
         g = _generator(key, dev)
@@ -204,8 +213,9 @@ def _opts(use_fixed_step_size, rtol, atol, step_size, solver, max_steps):
 # --------------------------------------------------------------------------------------------------
 def sample_cnf(cnf: FlowMatchingCNF, params: Params, key, features=None, use_fixed_step_size: bool = False,
                rtol: float = 1e-5, atol: float = 1e-5, step_size: float = 0.05, *, n_samples: Optional[int] = None,
-               x0=None, solver: str = "dopri5", max_steps: int = 4096):
-    """sample_and_log_prob.py:11-38: x0 ~ base, ODE 0 -> 1; returns x1 ([N*D] for one molecule, else [B, N*D])."""
+               x0=None, solver: str = "dopri5", max_steps: int = 4096, context=None):
+    """sample_and_log_prob.py:11-38: x0 ~ base, ODE 0 -> 1; returns x1 ([N*D] for one molecule, else [B, N*D]).
+    context: an ecnf_amd.context.Context the field's node embeddings read (here and in the functions below)."""
     cfg = cnf.cfg
     h = cnf.to_device(params)
     if x0 is not None:
@@ -216,13 +226,14 @@ def sample_cnf(cnf: FlowMatchingCNF, params: Params, key, features=None, use_fix
     else:
         feats, B, squeeze = _batched(features, cfg, n_samples)
         x0 = cnf.sample_base(key, B)
-    y1, _, _, _ = h.integrate(x0, feats, 0.0, 1.0, _opts(use_fixed_step_size, rtol, atol, step_size, solver, max_steps))
+    y1, _, _, _ = h.integrate(x0, feats, 0.0, 1.0, _opts(use_fixed_step_size, rtol, atol, step_size, solver, max_steps),
+                              node_embedding=_node_embedding(h, features, context))
     return y1[0] if squeeze else y1
 
 
 def get_log_prob(cnf: FlowMatchingCNF, params: Params, x, key, features=None, approx: bool = False,
                  use_fixed_step_size: bool = False, rtol: float = 1e-5, atol: float = 1e-5, step_size: float = 0.05,
-                 *, eps=None, solver: str = "dopri5", max_steps: int = 4096):
+                 *, eps=None, solver: str = "dopri5", max_steps: int = 4096, context=None):
     """sample_and_log_prob.py:41-94: ODE 1 -> 0 on (x, 0); returns (log_p, log_prob_base, delta_log_likelihood).
 
     approx=False: exact trace of the full N*D Jacobian; approx=True: Hutchinson with eps ~ N(0, I) drawn once."""
@@ -237,7 +248,8 @@ def get_log_prob(cnf: FlowMatchingCNF, params: Params, x, key, features=None, ap
         g = _generator(key, cnf.device)
         eps = torch.randn(x.shape, generator=g, device=cnf.device, dtype=torch.float32)
     x0, dl, _, _ = h.integrate(x, feats, 1.0, 0.0, _opts(use_fixed_step_size, rtol, atol, step_size, solver,
-                                                          max_steps), divergence=div, eps=eps)
+                                                          max_steps), divergence=div, eps=eps,
+                               node_embedding=_node_embedding(h, features, context))
     lpb = h.base_log_prob(x0)
     log_p = lpb + dl
     if squeeze:
@@ -248,7 +260,7 @@ def get_log_prob(cnf: FlowMatchingCNF, params: Params, x, key, features=None, ap
 def sample_and_log_prob_cnf(cnf: FlowMatchingCNF, params: Params, key, features=None, approx: bool = False,
                             use_fixed_step_size: bool = False, rtol: float = 1e-5, atol: float = 1e-5,
                             step_size: float = 0.05, *, n_samples: Optional[int] = None, z=None,
-                            solver: str = "dopri5", max_steps: int = 4096):
+                            solver: str = "dopri5", max_steps: int = 4096, context=None):
     """sample_and_log_prob.py:97-149: x0 ~ base, ODE 0 -> 1 on (x0, 0); returns (x1, log p0(x0) - l(1)).
 
     As in the reference, the Hutchinson probe is the same standard-normal draw z that produced x0
@@ -267,7 +279,8 @@ def sample_and_log_prob_cnf(cnf: FlowMatchingCNF, params: Params, key, features=
     x0 = h.base_sample(z)
     div = _lib.DIV_HUTCHINSON if approx else _lib.DIV_EXACT
     x1, dl, _, _ = h.integrate(x0, feats, 0.0, 1.0, _opts(use_fixed_step_size, rtol, atol, step_size, solver,
-                                                           max_steps), divergence=div, eps=z)
+                                                           max_steps), divergence=div, eps=z,
+                               node_embedding=_node_embedding(h, features, context))
     log_p = h.base_log_prob(x0) - dl
     if squeeze:
         return x1[0], log_p[0]

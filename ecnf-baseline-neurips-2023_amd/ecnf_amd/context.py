@@ -3,6 +3,11 @@
   * :func:`qk_norm_rotary` / :func:`qk_norm_rotary_grad`     per-head norm of queries and keys and the rotation by
     their positions (one to four axes, e.g. chain / residue / atom) in one pass        (ecnf_qk_norm_rotary)
   * :func:`cross_attention` / :func:`cross_attention_grad`   softmax(scale q k^T) v     (ecnf_cross_attention)
+  * :class:`Context`, :func:`node_embedding` / :func:`node_embedding_grad`: a conditional flow.  The embedding row of an
+    atom's feature also attends to the states; the result takes the row's place in the vector field
+    (``context=`` of ``cnf.apply``, ``sample_cnf``, ``get_log_prob``, ``sample_and_log_prob_cnf`` and
+    ``flow_matching_loss_fn``).  It reads no coordinates, so the field stays equivariant, and it is constant along the
+    ODE, so a solve computes it once.
 
 Tensors are [batch, length, heads, head_dim] in float32, bfloat16 or float16, on one device, with any strides (the last
 dimension contiguous, else it is copied first).  The calls run on the tensors' device and torch's current stream of
@@ -14,11 +19,13 @@ from __future__ import annotations
 
 import ctypes
 import struct
-from typing import Optional, Sequence, Tuple
+from dataclasses import dataclass
+from typing import Dict, Mapping, NamedTuple, Optional, Sequence, Tuple
 
 import torch
 
 from . import _lib
+from .params import CNFConfig
 
 _DTYPES = {torch.float32: _lib.DTYPE_F32, torch.bfloat16: _lib.DTYPE_BF16, torch.float16: _lib.DTYPE_F16}
 _POSITIONS = {torch.int32: _lib.POS_I32, torch.int64: _lib.POS_I64, torch.float32: _lib.POS_F32}
@@ -255,3 +262,122 @@ def cross_attention_grad(out_grad, q, k, v, out, lse, *, query_lengths=None, con
         dk.zero_()
         dv.zero_()
     return dq, dk, dv
+
+
+# ------------------------------------------------------------------------------------------------------ the conditional flow
+@dataclass(frozen=True)
+class ContextConfig:
+    """Attention from the atoms to states [.., state_dim]: n_heads query heads on n_kv_heads key heads of head_dim, turned
+    by positions on ``axes`` (:func:`qk_norm_rotary`)."""
+    state_dim: int
+    n_heads: int = 2
+    n_kv_heads: int = 2
+    head_dim: int = 32
+    axes: Tuple[int, ...] = (32,)
+    theta: float = 10000.0
+    eps: float = 1e-6
+    interleaved: bool = False
+
+
+class Context(NamedTuple):
+    """What a batch of molecules is conditioned on.  params: :func:`init_context_params`; states [C, Lk, state_dim] in
+    the dtype to compute in (C: the batch, or 1 for all of it); node_positions [N, n_axes] or [batch, N, n_axes] of the
+    atoms and positions [Lk, n_axes] or [C, Lk, n_axes] of the states (the same axes); lengths [C] and mask [C, Lk] as
+    in :func:`cross_attention`."""
+    cfg: ContextConfig
+    params: Mapping[str, torch.Tensor]
+    states: torch.Tensor
+    node_positions: torch.Tensor
+    positions: torch.Tensor
+    lengths: Optional[torch.Tensor] = None
+    mask: Optional[torch.Tensor] = None
+
+
+def _hidden(cnf_cfg: CNFConfig) -> int:
+    return cnf_cfg.ref_hidden or cnf_cfg.hidden
+
+
+def init_context_params(cfg: ContextConfig, cnf_cfg: CNFConfig, seed: int = 0, device=0) -> Dict[str, torch.Tensor]:
+    """Projections (fan-in scaled normal) and norm weights (1), fp32; the output projection is 0, so an untrained
+    context leaves the field as it is."""
+    dev = torch.device("cuda", device) if isinstance(device, int) else torch.device(device)
+    g = torch.Generator()
+    g.manual_seed(seed)
+    H, q, kv = _hidden(cnf_cfg), cfg.n_heads * cfg.head_dim, cfg.n_kv_heads * cfg.head_dim
+
+    def normal(rows, cols):
+        return (torch.randn((rows, cols), generator=g) * rows ** -0.5).to(dev)
+    return {"query": normal(H, q), "key": normal(cfg.state_dim, kv), "value": normal(cfg.state_dim, kv),
+            "out": torch.zeros((q, H), device=dev), "query_norm": torch.ones(cfg.head_dim, device=dev),
+            "key_norm": torch.ones(cfg.head_dim, device=dev)}
+
+
+def _project(x: torch.Tensor, w: torch.Tensor, heads: int) -> torch.Tensor:
+    """[B, L, F] @ [F, heads * D] -> [B, L, heads, D] in x's dtype"""
+    return (x.reshape(-1, x.shape[-1]) @ w.to(x.dtype)).reshape(x.shape[0], x.shape[1], heads, -1)
+
+
+def node_embedding(embedding: torch.Tensor, features, context: Context, cnf_cfg: CNFConfig,
+                   return_saved: bool = False):
+    """h_i = E[f_i] + W_out attention(norm_rotary(W_q E[f_i]), norm_rotary(W_k s), W_v s) for every atom i:
+    [batch, N, H] in fp32 (batch 1 where features are [N] and the context is shared: the same for every molecule).
+    embedding: the field's nn.Embed table [n_features, H] (``EcnfHandle.embedding``).  return_saved: also what
+    :func:`node_embedding_grad` takes."""
+    c, p = context.cfg, context.params
+    H, N = _hidden(cnf_cfg), cnf_cfg.n_nodes
+    s = context.states
+    if not (torch.is_tensor(s) and s.device == embedding.device and s.dim() == 3 and s.shape[2] == c.state_dim
+            and s.dtype in _DTYPES and s.shape[0] >= 1):
+        raise ValueError(f"states must be a floating [contexts, length, {c.state_dim}] tensor on {embedding.device}")
+    if features is None:
+        raise ValueError("features must be given for the EGNN vector field (build_cnf.py:73-75)")
+    f = torch.as_tensor(features)
+    if f.dtype.is_floating_point:
+        raise ValueError("features are integer embedding ids")
+    if not f.is_cuda and f.numel() and (int(f.min()) < 0 or int(f.max()) >= cnf_cfg.n_features):
+        raise ValueError(f"feature ids must lie in [0, {cnf_cfg.n_features})")
+    f = f.to(embedding.device).long()
+    if f.dim() == 1:
+        f = f[None].expand(s.shape[0], -1)
+    if f.dim() != 2 or f.shape[1] != N or s.shape[0] not in (1, f.shape[0]):
+        raise ValueError(f"features must be [{N}] or [batch, {N}] and states of the same batch or 1, got "
+                         f"{tuple(f.shape)} and {tuple(s.shape)}")
+    # device-resident ids are not read back: an id outside the table gives NaN rows, as elsewhere on the call path
+    known = ((f >= 0) & (f < cnf_cfg.n_features))[..., None]
+    e = embedding[:, :H][f.clamp(0, cnf_cfg.n_features - 1)]
+    e = torch.where(known, e, torch.full_like(e, float("nan")))
+    x = e.to(s.dtype)
+    q, k, v = (_project(x, p["query"], c.n_heads), _project(s, p["key"], c.n_kv_heads),
+               _project(s, p["value"], c.n_kv_heads))
+    turn = dict(q_positions=context.node_positions, k_positions=context.positions, q_weight=p["query_norm"],
+                k_weight=p["key_norm"], axes=c.axes, theta=c.theta, eps=c.eps, interleaved=c.interleaved)
+    qr, kr = qk_norm_rotary(q, k, **turn)
+    keep = dict(context_lengths=context.lengths, context_mask=context.mask)
+    o, lse = cross_attention(qr, kr, v, return_lse=True, **keep)
+    nodes = e + (o.reshape(-1, o.shape[2] * o.shape[3]) @ p["out"].to(o.dtype)).float().reshape(e.shape)
+    if not return_saved:
+        return nodes
+    return nodes, (f, x, s, q, k, v, qr, kr, o, lse, turn, keep, p, embedding.shape)
+
+
+def node_embedding_grad(d_nodes: torch.Tensor, saved) -> Dict[str, torch.Tensor]:
+    """Gradients of :func:`node_embedding` for the gradient of its result: {"embedding" (the table's), "states", and one
+    per context parameter}, each in its operand's dtype."""
+    f, x, s, q, k, v, qr, kr, o, lse, turn, keep, p, table = saved
+    rows = lambda t: t.reshape(t.shape[0] * t.shape[1], -1)                 # noqa: E731
+    d_nodes = d_nodes.float().reshape(x.shape)
+    dn = rows(d_nodes).to(o.dtype)
+    do = (dn @ p["out"].to(o.dtype).t()).reshape(o.shape)
+    dqr, dkr, dv = cross_attention_grad(do, qr, kr, v, o, lse, **keep)
+    dq, dk, dqn, dkn = qk_norm_rotary_grad(dqr, dkr, q, k, **turn)
+    g = {"query": rows(x).t() @ rows(dq), "key": rows(s).t() @ rows(dk), "value": rows(s).t() @ rows(dv),
+         "out": rows(o).t() @ dn, "query_norm": dqn, "key_norm": dkn}
+    g = {n: t.to(p[n].dtype) for n, t in g.items()}
+    g["states"] = (rows(dk) @ p["key"].to(s.dtype).t() + rows(dv) @ p["value"].to(s.dtype).t()).reshape(s.shape)
+    de = d_nodes + (rows(dq) @ p["query"].to(x.dtype).t()).float().reshape(x.shape)
+    # the table's rows: one product with the features' indicator (a fixed order of sums, unlike a scatter)
+    hot = (rows(f[..., None]) == torch.arange(table[0], device=f.device)).to(torch.float32)
+    emb = torch.zeros(table, device=f.device, dtype=torch.float32)
+    emb[:, :x.shape[-1]] = hot.t() @ rows(de)
+    g["embedding"] = emb
+    return g

@@ -47,6 +47,20 @@ class SolveOptions:
         return o
 
 
+def pad_nodes(e, cfg: CNFConfig, device) -> torch.Tensor:
+    """Node embeddings [N, H] or [B, N, H] of the network's width (the reference's, for a zero-padded config) as fp32
+    [B, N, cfg.hidden]: padded columns are zero, as in padded parameters."""
+    e = torch.as_tensor(e, device=device, dtype=torch.float32)
+    if e.dim() == 2:
+        e = e[None]
+    widths = (cfg.hidden, cfg.ref_hidden) if cfg.ref_hidden else (cfg.hidden,)
+    if e.dim() != 3 or e.shape[1] != cfg.n_nodes or e.shape[2] not in widths:
+        raise ValueError(f"node_embedding must be [batch, {cfg.n_nodes}, {widths[-1]}], got {tuple(e.shape)}")
+    if e.shape[2] < cfg.hidden:
+        e = torch.nn.functional.pad(e, (0, cfg.hidden - e.shape[2]))
+    return e.contiguous()
+
+
 PRECISIONS = {"split_f16": _lib.PREC_SPLIT_F16, "fp32": _lib.PREC_FP32}
 
 
@@ -77,6 +91,7 @@ class EcnfHandle:
         _lib.check(self.lib.ecnf_create(ctypes.byref(self._c), blob.ctypes.data, blob.size, self.device.index,
                                         ctypes.byref(h)))
         self._h = h
+        self._set_embedding(blob)
         # callbacks run when this handle's weights or precision change (ecnf_amd.cnf evicts its content-hash cache
         # entry, so a params dict never maps to a handle holding other weights)
         self._on_mutate = []
@@ -87,6 +102,12 @@ class EcnfHandle:
             self.precision = "fp32"
         else:
             self._set_precision(precision)
+
+    def _set_embedding(self, blob) -> None:
+        # the nn.Embed table [n_features, hidden] (the last entry of the flat blob): the context operators' queries
+        n = self.cfg.n_features * self.cfg.hidden
+        self.embedding = torch.as_tensor(blob[-n:], device=self.device).clone().reshape(self.cfg.n_features,
+                                                                                        self.cfg.hidden)
 
     def _mutated(self) -> None:
         for cb in self._on_mutate:
@@ -102,6 +123,7 @@ class EcnfHandle:
             if p.numel() != param_count(self.cfg):
                 raise ValueError(f"params blob has {p.numel()} floats, expected {param_count(self.cfg)}")
             _lib.check(self.lib.ecnf_update_params(self._h, p.data_ptr(), 1))
+            self._set_embedding(p)
             self._sync_precision()
             return
         blob = params if isinstance(params, np.ndarray) else flatten_params(params, self.cfg)
@@ -109,6 +131,7 @@ class EcnfHandle:
         if blob.size != param_count(self.cfg):
             raise ValueError(f"params blob has {blob.size} floats, expected {param_count(self.cfg)}")
         _lib.check(self.lib.ecnf_update_params(self._h, blob.ctypes.data, 0))
+        self._set_embedding(blob)
         self._sync_precision()
 
     def _sync_precision(self) -> None:
@@ -168,6 +191,16 @@ class EcnfHandle:
             raise ValueError(f"features must have {N} entries per molecule")
         return f.reshape(batch, N).to(torch.int32).contiguous()
 
+    def _nodes(self, e, batch):
+        """Node embeddings [N, H], [1, N, H] (the same for every molecule) or [batch, N, H] -> (table [rows, hidden],
+        row ids [batch, N])."""
+        e = pad_nodes(e, self.cfg, self.device)
+        N = self.cfg.n_nodes
+        if e.shape[0] not in (1, batch):
+            raise ValueError(f"node_embedding must have 1 or {batch} molecules, got {e.shape[0]}")
+        row = torch.arange(e.shape[0] * N, device=self.device, dtype=torch.int32).reshape(-1, N)
+        return e.reshape(-1, self.cfg.hidden), row.expand(batch, N).contiguous()
+
     def molecules_per_workgroup(self, with_tangent: bool = False) -> int:
         v = ctypes.c_int32()
         _lib.check(self.lib.ecnf_molecules_per_workgroup(self._h, int(with_tangent), ctypes.byref(v)))
@@ -191,11 +224,18 @@ class EcnfHandle:
         return {_lib.CHAIN_SPLIT_BF16: "split_bf16", _lib.CHAIN_SPLIT_F16: "split_f16"}.get(v.value, "fp32_mfma")
 
     # ---------------------------------------------------------------------------------- C-ABI calls
-    def vector_field(self, x, t, feat) -> torch.Tensor:
-        """cnf.apply(params, x[B, N*D], t[B], features[B, N]) (core.py:7-19)."""
+    def vector_field(self, x, t, feat=None, *, node_embedding=None) -> torch.Tensor:
+        """cnf.apply(params, x[B, N*D], t[B], features[B, N]) (core.py:7-19); node_embedding [B or 1, N, H] takes the
+        place of the embedded features (ecnf_vector_field_nodes)."""
         x = self._f32(x, (self.cfg.event_dim,), "x")
         B = x.shape[0]
         t = torch.as_tensor(t, device=self.device, dtype=torch.float32).reshape(-1).expand(B).contiguous()
+        if node_embedding is not None:
+            nodes, row = self._nodes(node_embedding, B)
+            v = torch.empty_like(x)
+            _lib.check(self.lib.ecnf_vector_field_nodes(self._h, _ptr(x), _ptr(t), _ptr(nodes), nodes.shape[0], _ptr(row),
+                                                        _ptr(v), B, _stream(self.device)))
+            return v
         f = self._feat(feat, B)
         v = torch.empty_like(x)
         _lib.check(self.lib.ecnf_vector_field(self._h, _ptr(x), _ptr(t), _ptr(f), _ptr(v), B, _stream(self.device)))
@@ -220,7 +260,7 @@ class EcnfHandle:
         return v, ju
 
     def integrate(self, y0, feat, t0: float, t1: float, opts: SolveOptions, divergence: int = _lib.DIV_NONE,
-                  eps=None, check_status: bool = True, fallback: bool = True):
+                  eps=None, check_status: bool = True, fallback: bool = True, *, node_embedding=None):
         """ODE solve of the whole batch in one launch (adaptive solves with more workgroups than CUs: two launches,
         the unfinished molecules re-dealt longest first; bitwise the same results).  Returns (y1, dlogp or None, nfe,
         status).
@@ -229,10 +269,11 @@ class EcnfHandle:
         ECNF_E_MAX_STEPS -> RuntimeError, ECNF_E_INVALID (embedding ids out of range) -> ValueError.
         fallback (with check_status, split_f16 precision): molecules that report ECNF_E_NONFINITE (an activation
         beyond the fp16 range of the split GEMMs) are solved again on the strict-fp32 kernels and replaced; a
-        molecule that is still non-finite raises."""
+        molecule that is still non-finite raises.
+        node_embedding [B or 1, N, H]: takes the place of the embedded features (feat is not read)."""
         y0 = self._f32(y0, (self.cfg.event_dim,), "y0")
         B = y0.shape[0]
-        f = self._feat(feat, B)
+        nodes, f = (None, self._feat(feat, B)) if node_embedding is None else self._nodes(node_embedding, B)
         e = None
         if divergence == _lib.DIV_HUTCHINSON:
             if eps is None:
@@ -240,7 +281,7 @@ class EcnfHandle:
             e = self._f32(eps, (self.cfg.event_dim,), "eps")
             if e.shape[0] != B:
                 raise ValueError("eps batch mismatch")
-        y1, dl, nfe, status = self._integrate(y0, f, e, t0, t1, opts, divergence)
+        y1, dl, nfe, status = self._integrate(y0, f, e, t0, t1, opts, divergence, nodes)
         if check_status and B:
             bad = status != _lib.ECNF_OK
             if bool(bad.any()):
@@ -251,7 +292,8 @@ class EcnfHandle:
                     self._set_precision("fp32")
                     try:
                         r = self._integrate(y0[idx].contiguous(), f[idx].contiguous(),
-                                            None if e is None else e[idx].contiguous(), t0, t1, opts, divergence)
+                                            None if e is None else e[idx].contiguous(), t0, t1, opts, divergence,
+                                            nodes)
                     finally:
                         self._set_precision("split_f16")
                     y1[idx], nfe[idx], status[idx] = r[0], r[2], r[3]
@@ -272,7 +314,7 @@ class EcnfHandle:
                     raise RuntimeError(f"{n_hip} molecule(s) failed on the device (a team exchange timed out)")
         return y1, dl, nfe, status
 
-    def _integrate(self, y0, f, e, t0, t1, opts: SolveOptions, divergence: int):
+    def _integrate(self, y0, f, e, t0, t1, opts: SolveOptions, divergence: int, nodes=None):
         B = y0.shape[0]
         y1 = torch.empty_like(y0)
         dl = torch.empty(B, device=self.device, dtype=torch.float32) if divergence != _lib.DIV_NONE else None
@@ -285,6 +327,11 @@ class EcnfHandle:
         nbytes = ctypes.c_size_t(0)
         _lib.check(self.lib.ecnf_integrate_workspace_size(self._h, ctypes.byref(o), B, ctypes.byref(nbytes)))
         ws = torch.empty(nbytes.value, device=self.device, dtype=torch.uint8) if nbytes.value else None
+        if nodes is not None:
+            _lib.check(self.lib.ecnf_integrate_nodes(self._h, ctypes.byref(o), _ptr(y0), _ptr(nodes), nodes.shape[0],
+                                                     _ptr(f), _ptr(e), _ptr(y1), _ptr(dl), _ptr(nfe), _ptr(status), B,
+                                                     _ptr(ws), nbytes.value, _stream(self.device)))
+            return y1, dl, nfe, status
         _lib.check(self.lib.ecnf_integrate_ws(self._h, ctypes.byref(o), _ptr(y0), _ptr(f), _ptr(e), _ptr(y1), _ptr(dl),
                                               _ptr(nfe), _ptr(status), B, _ptr(ws), nbytes.value,
                                               _stream(self.device)))

@@ -21,6 +21,7 @@ import numpy as np
 import torch
 
 from . import _lib
+from .engine import pad_nodes
 from .params import CNFConfig, flatten_params, param_count
 
 
@@ -103,6 +104,33 @@ class Trainer:
         _lib.check(self.lib.ecnf_fm_loss_grad(self._h, _ptr(p), _ptr(x1), _ptr(x0), _ptr(t), _ptr(f), sm, B,
                                               _ptr(loss), _ptr(grad), self._stream()))
         return loss[0], grad
+
+    def loss_and_grad_nodes(self, params: torch.Tensor, x1, x0, t, node_embedding, sigma_min: Optional[float] = None):
+        """(loss, grad, node gradient) of the same loss with node embeddings [B or 1, N, H] in place of the embedded
+        features (ecnf_fm_loss_grad_nodes): grad's embedding table is 0, the node gradient has node_embedding's shape
+        (summed over the batch where it is shared)."""
+        cfg = self.cfg
+        p = self.device_params(params)
+        x1 = torch.as_tensor(x1, device=self.device, dtype=torch.float32).reshape(-1, cfg.event_dim).contiguous()
+        B = x1.shape[0]
+        if B < 1 or B > self.max_batch:
+            raise ValueError(f"batch must lie in [1, {self.max_batch}]")
+        x0 = torch.as_tensor(x0, device=self.device, dtype=torch.float32).reshape(B, cfg.event_dim).contiguous()
+        t = torch.as_tensor(t, device=self.device, dtype=torch.float32).reshape(B).contiguous()
+        shape = tuple(node_embedding.shape)
+        e = pad_nodes(node_embedding, cfg, self.device)
+        if e.shape[0] not in (1, B):
+            raise ValueError(f"node_embedding must have 1 or {B} molecules, got {e.shape[0]}")
+        nodes = e.expand(B, -1, -1).contiguous()
+        loss = torch.empty(1, device=self.device, dtype=torch.float32)
+        grad = torch.empty(self.n_params, device=self.device, dtype=torch.float32)
+        dn = torch.empty_like(nodes)
+        sm = cfg.sigma_min if sigma_min is None else float(sigma_min)
+        _lib.check(self.lib.ecnf_fm_loss_grad_nodes(self._h, _ptr(p), _ptr(x1), _ptr(x0), _ptr(t), _ptr(nodes), sm, B,
+                                                    _ptr(loss), _ptr(grad), _ptr(dn), self._stream()))
+        if e.shape[0] != B:
+            dn = dn.sum(0, keepdim=True)
+        return loss[0], grad, dn[..., :shape[-1]].reshape(shape)
 
     def adam_update(self, grad, params, mu, nu, ema, lr: float, count: int, b1: float = 0.9, b2: float = 0.999,
                     eps: float = 1e-8, eps_root: float = 0.0, ema_beta: float = 0.999):
@@ -210,8 +238,11 @@ def _noise(cnf, key, batch: int):
     return x0, t
 
 
-def flow_matching_loss_fn(cnf, params, x_data, key, features=None, *, x0=None, t=None, with_grad: bool = False):
-    """loss.py:10-32: (loss, info).  with_grad=True returns (loss, info, grad) -- jax.grad's companion here."""
+def flow_matching_loss_fn(cnf, params, x_data, key, features=None, *, x0=None, t=None, with_grad: bool = False,
+                          context=None):
+    """loss.py:10-32: (loss, info).  with_grad=True returns (loss, info, grad) -- jax.grad's companion here.
+    context (ecnf_amd.context.Context): the field's node embeddings also read it; info["context_grad"] then holds the
+    gradients of its parameters and states."""
     if features is None:
         raise ValueError("features must be given for the EGNN vector field (build_cnf.py:73-75)")
     x_data = torch.as_tensor(x_data, device=cnf.device, dtype=torch.float32)
@@ -223,8 +254,20 @@ def flow_matching_loss_fn(cnf, params, x_data, key, features=None, *, x0=None, t
         x0 = nx0 if x0 is None else x0
         t = nt if t is None else t
     tr = trainer_for(cnf.cfg, B, cnf.device)
-    loss, grad = tr.loss_and_grad(params, x_data, x0, t, features)
-    info = {"loss": loss}
+    if context is None:
+        loss, grad = tr.loss_and_grad(params, x_data, x0, t, features)
+        info = {"loss": loss}
+    else:
+        from . import context as C
+        p, n = tr.device_params(params), cnf.cfg.n_features * cnf.cfg.hidden
+        embedding = p[-n:].reshape(cnf.cfg.n_features, cnf.cfg.hidden)
+        nodes, saved = C.node_embedding(embedding, features, context, cnf.cfg, return_saved=True)
+        loss, grad, dn = tr.loss_and_grad_nodes(p, x_data, x0, t, nodes)
+        info = {"loss": loss}
+        if with_grad:
+            cg = C.node_embedding_grad(dn, saved)
+            grad[-n:] = cg.pop("embedding").reshape(-1)
+            info["context_grad"] = cg
     return (loss, info, grad) if with_grad else (loss, info)
 
 

@@ -124,6 +124,16 @@ int ecnf_integrate(ecnf_handle* h, const ecnf_solve_opts* opts, const float* y0,
                    const float* eps, float* y1, float* dlogp, int32_t* nfe, int32_t* status, int32_t batch,
                    void* stream);
 
+/* ecnf_vector_field / ecnf_integrate_ws with the call's own node embeddings in place of the nn.Embed rows (a field
+ * conditioned on a context: ecnf_amd.context): nodes [n_rows, hidden] (DEVICE, fp32), row [batch, N] ids in [0, n_rows)
+ * (checked like embedding ids).  With nodes = the embedding table and row = feat the results are those of the calls
+ * above (for one-feature 13-atom molecules up to the rounding of the block-1 pair tiles, which need equal rows). */
+int ecnf_vector_field_nodes(ecnf_handle* h, const float* x, const float* t, const float* nodes, int32_t n_rows,
+                            const int32_t* row, float* v, int32_t batch, void* stream);
+int ecnf_integrate_nodes(ecnf_handle* h, const ecnf_solve_opts* opts, const float* y0, const float* nodes,
+                         int32_t n_rows, const int32_t* row, const float* eps, float* y1, float* dlogp, int32_t* nfe,
+                         int32_t* status, int32_t batch, void* workspace, size_t workspace_bytes, void* stream);
+
 /* Device workspace of a solve.  The exact trace (ECNF_DIV_EXACT) runs N*D - D JVP passes per evaluation whose
  * primal is the same; with a workspace, the first pass caches the primal edge aggregates of the blocks whose edge
  * tangents are sparse (blocks 1 and K) and the later passes skip those primal tiles.  Results are bitwise equal with
@@ -250,6 +260,12 @@ int ecnf_trainer_set_reduction_arena(ecnf_trainer* tr, size_t floats, size_t* us
 int ecnf_fm_loss_grad(ecnf_trainer* tr, const float* params, const float* x1, const float* x0, const float* t,
                       const int32_t* feat, float sigma_min, int32_t batch, float* loss, float* grad, void* stream);
 
+/* ecnf_fm_loss_grad with node embeddings [batch, N, hidden] of the call's own: also writes their gradient (same shape);
+ * grad's embedding table entries are 0. */
+int ecnf_fm_loss_grad_nodes(ecnf_trainer* tr, const float* params, const float* x1, const float* x0, const float* t,
+                            const float* nodes, float sigma_min, int32_t batch, float* loss, float* grad,
+                            float* nodes_grad, void* stream);
+
 /* optax.adam(lr, b1, b2, eps, eps_root) at step `count` (1 for the first update: the bias corrections use
  * 1 - b^count) applied in place: params += -lr mu_hat / (sqrt(nu_hat + eps_root) + eps); ema (optional, may be
  * NULL) = ema * ema_beta + (1 - ema_beta) * params.  norms (optional): DEVICE float[2] = (|grad|, |update|), the
@@ -267,7 +283,7 @@ int ecnf_update_params(ecnf_handle* h, const float* params, int32_t on_device);
 
 /* ---- context operators (no handle needed): attention from the atoms to an encoder's states of another length ----
  * The reference's field knows its molecule by an embedded id per atom only; these operators make a node embedding that
- * also reads a context (ecnf_amd.context; ecnf_integrate_nodes and its kin take it).
+ * also reads a context (ecnf_amd.context); ecnf_integrate_nodes and its kin take that.
  *   - tensors are [batch, length, heads, head_dim] in any of ecnf_dtype; strides in elements for the first three
  *     dimensions, the last one contiguous; outputs and gradients are contiguous.
  *   - `device` is the operands' device: it is made current for the launches and the caller's restored.

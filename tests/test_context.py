@@ -128,3 +128,12 @@ def test_host_tensors_are_refused():
         context.cross_attention(q, q, q)
     with pytest.raises(ValueError, match="device"):
         context.qk_norm_rotary(q, q_positions=torch.zeros(2, 1), axes=(16,))
+
+
+def test_node_entries_refuse_missing_handles():
+    lib = _lib.load()
+    assert lib.ecnf_vector_field_nodes(None, None, None, None, 1, None, None, 1, None) == _lib.ECNF_E_INVALID
+    assert lib.ecnf_integrate_nodes(None, None, None, None, 1, None, None, None, None, None, None, 1, None, 0,
+                                    None) == _lib.ECNF_E_INVALID
+    assert lib.ecnf_fm_loss_grad_nodes(None, None, None, None, None, None, 0.0, 1, None, None, None,
+                                       None) == _lib.ECNF_E_INVALID
