@@ -39,6 +39,11 @@ typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
 #define ECNF_LDS(T) __attribute__((address_space(3))) T
 
+template <int V>
+struct Const {
+  static constexpr int value = V;
+};
+
 constexpr float kInf = __builtin_inff();
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
@@ -65,6 +70,7 @@ struct Att {
   int32_t R;                       // rows of a (context, key head): per * Lq * G
   int32_t tiles;                   // row or key tiles of a (context, key head)
   int32_t splits;
+  int32_t flat;                    // tokens of a context are one sequence in q and dout (see RowTile)
   float scale;
 };
 
@@ -77,7 +83,7 @@ struct Ops<__bf16> {
   static __device__ __forceinline__ f32x16 mma(Frag a, Frag b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
   }
-  static __device__ __forceinline__ Quad tr(ECNF_LDS(char) * p) {
+  static __device__ __forceinline__ Quad tr(uint32_t p) {
     return __builtin_amdgcn_ds_read_tr16_b64_v4bf16((ECNF_LDS(bf16x4)*)p);
   }
 };
@@ -88,7 +94,7 @@ struct Ops<_Float16> {
   static __device__ __forceinline__ f32x16 mma(Frag a, Frag b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
   }
-  static __device__ __forceinline__ Quad tr(ECNF_LDS(char) * p) {
+  static __device__ __forceinline__ Quad tr(uint32_t p) {
     typedef __fp16 h4 __attribute__((ext_vector_type(4)));
     return __builtin_bit_cast(f16x4, __builtin_amdgcn_ds_read_tr16_b64_v4f16((ECNF_LDS(h4)*)p));
   }
@@ -134,40 +140,55 @@ struct Tile {
   static constexpr int kRow = DP * (int)sizeof(T);   // bytes
   static constexpr int kChunks = kRow / 16;
   static constexpr int kPer = 16 / (int)sizeof(T);   // elements of a chunk
-  static __device__ __forceinline__ int f(int r) {
+  static constexpr __host__ __device__ __forceinline__ int f(int r) {
     if constexpr (kChunks >= 16) return ((r & 3) << 2) | ((r >> 2) & 3);
     else if constexpr (kChunks == 8) return ((r & 2) << 1) | ((r >> 2) & 3);
     else return (r >> 2) & 3;
   }
   static __device__ __forceinline__ int at(int r, int c) { return r * kRow + ((c ^ f(r)) << 4); }
+};
 
-  // operand of a 16-deep step s: 8 elements 16 s + 8 h .. of row r
-  static __device__ __forceinline__ typename Ops<T>::Frag frag(const char* t, int r, int s, int h) {
-    typedef typename Ops<T>::Frag Frag;
-    if constexpr (sizeof(T) == 2) {
-      return *reinterpret_cast<const Frag*>(t + at(r, 2 * s + h));
-    } else {
-      const f32x4 a = *reinterpret_cast<const f32x4*>(t + at(r, 4 * s + 2 * h));
-      const f32x4 b = *reinterpret_cast<const f32x4*>(t + at(r, 4 * s + 2 * h + 1));
-      return Frag{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
-    }
-  }
-  // operand of the transposed product: column d0 + l % 32, rows r0 + {4h .. 4h+3, 8+4h .. 8+4h+3}
-  static __device__ __forceinline__ typename Ops<T>::Frag frag_t(char* t, int r0, int d0, int l) {
-    typename Ops<T>::Frag o;
+// A lane's reads of tiles.  f only permutes bits, so every address is the lane's base with constant bits turned
+// (one instruction) plus a constant offset: nothing but two bases stays in registers.
+template <class T, int DP>
+struct Reader {
+  typedef Tile<T, DP> TL;
+  typedef typename Ops<T>::Frag Frag;
+  uint32_t fb, tb;
+  // l: lane; base: LDS address of the first tile (a multiple of 512, like every tile's)
+  __device__ __forceinline__ void init(uint32_t base, int l) {
     const int h = l >> 5;
     if constexpr (sizeof(T) == 2) {
-      const int r = r0 + 4 * h + ((l & 15) >> 2), d = d0 + (l & 16) + 4 * (l & 3);
-      const auto lo = Ops<T>::tr((ECNF_LDS(char)*)(t + at(r, d >> 3) + 2 * (d & 7)));
-      const auto hi = Ops<T>::tr((ECNF_LDS(char)*)(t + at(r + 8, d >> 3) + 2 * (d & 7)));
+      fb = base + TL::at(l & 31, h);
+      tb = base + TL::at(4 * h + ((l & 15) >> 2), ((l & 16) >> 3) | ((l & 3) >> 1)) + 8 * (l & 1);
+    } else {
+      fb = base + TL::at(l & 31, 2 * h);
+      tb = base + TL::at(4 * h, (l & 31) >> 2) + 4 * (l & 3);
+    }
+  }
+  // operand of a 16-deep step s: elements 16 s + 8 h .. + 7 of row r0 + l % 32 (r0 a multiple of 32) of the tile at `at`
+  __device__ __forceinline__ Frag frag(uint32_t at, int r0, int s) const {
+    if constexpr (sizeof(T) == 2) {
+      return *(ECNF_LDS(const Frag)*)(((fb + at) ^ (uint32_t)(s << 5)) + r0 * TL::kRow);
+    } else {
+      const uint32_t p = ((fb + at) ^ (uint32_t)(s << 6)) + r0 * TL::kRow, q = ((fb + at) ^ (uint32_t)(s << 6 | 16)) + r0 * TL::kRow;
+      const f32x4 x = *(ECNF_LDS(const f32x4)*)p, y = *(ECNF_LDS(const f32x4)*)q;
+      return Frag{x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
+    }
+  }
+  // operand of the transposed product: column 32 d + l % 32 of the rows r0 + {4h .. 4h+3, 8+4h .. 8+4h+3} (r0 % 16 = 0)
+  __device__ __forceinline__ Frag frag_t(uint32_t at, int r0, int d) const {
+    Frag o;
+    if constexpr (sizeof(T) == 2) {
+      const auto lo = Ops<T>::tr(((tb + at) ^ (uint32_t)(d << 6)) + r0 * TL::kRow);
+      const auto hi = Ops<T>::tr(((tb + at) ^ (uint32_t)(d << 6 ^ TL::f(8) << 4)) + (r0 + 8) * TL::kRow);
 #pragma unroll
       for (int e = 0; e < 4; ++e) o[e] = lo[e], o[4 + e] = hi[e];
     } else {
-      const int d = d0 + (l & 31);
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const int r = r0 + 4 * h + (e & 3) + 8 * (e >> 2);
-        o[e] = *reinterpret_cast<const float*>(t + at(r, d >> 2) + 4 * (d & 3));
+        const int r = (e & 3) + 8 * (e >> 2);
+        o[e] = *(ECNF_LDS(const float)*)(((tb + at) ^ (uint32_t)(d << 7 ^ TL::f(r) << 4)) + (r0 + r) * TL::kRow);
       }
     }
     return o;
@@ -195,29 +216,113 @@ __device__ __forceinline__ void row_of(const Att& a, int c, int r, int& b, int& 
 }
 __device__ __forceinline__ bool row_live(const Att& a, int b, int i) { return !a.qlen || i < a.qlen[b]; }
 
-// The rows [r0, r0 + ROWS) of an operand as 16-byte chunks, NT threads: global -> registers -> LDS tile.  Rows outside
-// their range (and masked keys) are zeros whatever memory holds there, so NaN or infinity behind a mask never enters a
-// product; columns behind D (padding to the tile's DP) are zeros too.
-template <class T, int DP, int ROWS, int NT>
-struct Stage {
+// Tiles go from memory to LDS without passing registers (16-byte LDS loads): a wave's 64 chunks land consecutively, so
+// the lane that fills slot c' of row r asks for chunk c' ^ f(r).  Issued through asm (the compiler would otherwise make
+// every later LDS read wait for them); dma_wait before the barrier that publishes them.
+__device__ __forceinline__ void dma_buffer(uint32_t lds, u32x4 rsrc, uint32_t off) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(off), "s"(rsrc)
+               : "memory", "m0");
+}
+__device__ __forceinline__ void dma_global(uint32_t lds, const char* p) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(p) : "memory", "m0");
+}
+__device__ __forceinline__ void dma_wait() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+__device__ __forceinline__ uint32_t lds_address(const void* p) { return (uint32_t)(uintptr_t)(ECNF_LDS(const void)*)p; }
+__device__ __forceinline__ int wave_id() { return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); }
+
+// A tile of ROWS keys: constant stride, so one buffer descriptor a tile (its range ends behind the last valid row) and
+// lane offsets that stay the same from tile to tile.  What lies behind the range reads as zero, and a masked key's lanes
+// ask behind the range: NaN or infinity behind a length or mask never enters a product.  Columns behind D are zero too.
+constexpr uint32_t kBehind = 0x80000000u;
+template <class T, int DP, int ROWS>
+struct KeyTile {
   static constexpr int kCh = Tile<T, DP>::kChunks;
-  static constexpr int kN = (ROWS * kCh + NT - 1) / NT;
-  u32x4 x[kN];
-  template <class Addr>
-  __device__ __forceinline__ void load(int tid, int D, Addr addr) {
+  static constexpr int kN = ROWS * kCh / 256;       // chunks a thread
+  static constexpr int kStep = 256 / kCh;           // rows from one to the next
+  static constexpr int kAlt = kCh == 32 ? 2 : 1;    // f repeats every 16 rows
+  static_assert(kN >= 1 && ROWS * kCh % 256 == 0 && kStep * kAlt % 16 == 0, "whole chunks of a workgroup");
+  const char* base;
+  uint32_t stride, off[kAlt];
+  int row, end;   // end: bytes of a row
+  __device__ __forceinline__ void init(const char* b, int64_t row_stride, int D, int tid) {
+    base = b;
+    stride = (uint32_t)row_stride;
+    end = D * (int)sizeof(T);
+    row = tid / kCh;
 #pragma unroll
-    for (int n = 0; n < kN; ++n) {
-      const int id = tid + n * NT, r = id / kCh, c = id % kCh;
-      const char* p = (ROWS * kCh % NT == 0 || r < ROWS) && c * Tile<T, DP>::kPer < D ? addr(r) : nullptr;
-      x[n] = u32x4{0, 0, 0, 0};
-      if (p) x[n] = *reinterpret_cast<const u32x4*>(p + c * 16);
+    for (int x = 0; x < kAlt; ++x) {
+      const int c = ((tid % kCh) ^ Tile<T, DP>::f(row + x * kStep)) * 16;
+      off[x] = c < end ? (row + x * kStep) * stride + c : kBehind;
     }
   }
-  __device__ __forceinline__ void store(char* t, int tid) const {
+  template <class Allowed>
+  __device__ __forceinline__ void load(uint32_t lds, int k0, int valid, bool masked, Allowed allowed) const {
+    const uint64_t p = (uint64_t)(base + (int64_t)k0 * stride);
+    const int rows = min(valid, ROWS);
+    const u32x4 rsrc = {(uint32_t)p, (uint32_t)(p >> 32) & 0xffffu, (uint32_t)(rows - 1) * stride + (uint32_t)end, 0x00020000u};
+    const uint32_t at = lds + wave_id() * 1024;
 #pragma unroll
     for (int n = 0; n < kN; ++n) {
-      const int id = tid + n * NT, r = id / kCh, c = id % kCh;
-      if (ROWS * kCh % NT == 0 || r < ROWS) *reinterpret_cast<u32x4*>(t + Tile<T, DP>::at(r, c)) = x[n];
+      uint32_t o = off[n % kAlt] + (uint32_t)(n / kAlt * kAlt * kStep) * stride;
+      if (masked) o = allowed(k0 + row + n * kStep) ? o : kBehind;
+      dma_buffer(at + n * 4096, rsrc, o);
+    }
+  }
+};
+
+static __device__ const u32x4 kZeroRow[32] = {};   // 512 bytes: the longest row
+
+// A tile of ROWS query rows.  Fast form: a tile is whole tokens (G divides ROWS), the tokens of a context are evenly
+// spaced (a.flat) and none is behind a length, so like a key tile it is a descriptor that moves from tile to tile and
+// fixed lane offsets; only rows behind the last one turn to zero.  General form: an address a row, zeros from kZeroRow.
+template <class T, int DP, int ROWS>
+struct RowTile {
+  typedef Tile<T, DP> TL;
+  static constexpr int kCh = TL::kChunks;
+  static constexpr int kN = (ROWS * kCh + 255) / 256;
+  static_assert(ROWS * kCh % 64 == 0, "whole chunks of a wave");
+  const char* base;
+  int64_t s0, s1, s2;   // bytes
+  uint32_t off[kN];
+  __device__ __forceinline__ static int row(int n, int tid) { return (tid + n * 256) / kCh; }
+  __device__ __forceinline__ static bool mine(int n) { return ROWS * kCh % 256 == 0 || n * 256 + wave_id() * 64 < ROWS * kCh; }
+  __device__ __forceinline__ void init(const Att& a, const char* p, const int64_t* st, int c, int hk, int tid, bool fast) {
+    constexpr int64_t e = (int64_t)sizeof(T);
+    s0 = st[0] * e, s1 = st[1] * e, s2 = st[2] * e;
+    base = p + (int64_t)hk * a.G * s2 + (int64_t)c * a.per * s0;
+#pragma unroll
+    for (int n = 0; n < kN; ++n) {
+      const int r = row(n, tid), ch = ((tid + n * 256) % kCh) ^ TL::f(r);
+      const int t = (int)a.dG.div((uint32_t)r), g = r - t * a.G;
+      const uint32_t o = (fast ? (uint32_t)t * (uint32_t)s1 + (uint32_t)g * (uint32_t)s2 : 0u) + ch * 16;
+      off[n] = ch * TL::kPer < a.D ? o : kBehind;
+    }
+  }
+  // rows r0 .. of context c into the tile at `lds`
+  __device__ __forceinline__ void load(const Att& a, uint32_t lds, int c, int r0, int tid, bool fast) const {
+    const uint32_t at = lds + wave_id() * 1024;
+    if (fast) {
+      const uint64_t p = (uint64_t)(base + (int64_t)a.dG.div((uint32_t)r0) * s1);
+      const u32x4 rsrc = {(uint32_t)p, (uint32_t)(p >> 32) & 0xffffu, 0x7ffffff0u, 0x00020000u};
+      const bool tail = r0 + ROWS > a.R;
+#pragma unroll
+      for (int n = 0; n < kN; ++n) {
+        if (!mine(n)) break;
+        uint32_t o = off[n];
+        if (tail) o = r0 + row(n, tid) < a.R ? o : kBehind;
+        dma_buffer(at + n * 4096, rsrc, o);
+      }
+    } else {
+#pragma unroll
+      for (int n = 0; n < kN; ++n) {
+        if (!mine(n)) break;
+        const int r = min(r0 + row(n, tid), a.R - 1);
+        int b, i, g;
+        row_of(a, 0, r, b, i, g);
+        const bool ok = off[n] != kBehind && r0 + row(n, tid) < a.R && row_live(a, c * a.per + b, i);
+        const char* x = base + (int64_t)b * s0 + (int64_t)i * s1 + (int64_t)g * s2 + off[n];
+        dma_global(at + n * 4096, ok ? x : reinterpret_cast<const char*>(kZeroRow));
+      }
     }
   }
 };
@@ -258,19 +363,27 @@ template <class T, int DP, int WR, int WK, int KT>
 struct FwdShape {
   static constexpr int kKeys = WK * KT;
   static constexpr int kTileBytes = kKeys * DP * (int)sizeof(T);
-  static constexpr int kJoin = WK > 1 ? 4 * 32 * DP * 4 + 4 * 64 * 4 : 0;   // O of every wave, then m and l
-  static constexpr int kLds = (2 * kTileBytes + kKeys * 4 > kJoin ? 2 * kTileBytes + kKeys * 4 : kJoin);
+  // two buffers of K, V and the keys' bias; where the waves split the keys, the join reuses them: O of every wave, m, l
+  static constexpr int kBuf = 2 * kTileBytes;
+  static constexpr int kBufs = 2 * (kBuf + kKeys * 4) <= 160 * 1024 ? 2 : 1;
+  static constexpr int kBias = kBufs * kBuf;   // the biases lie behind the tiles (which start on multiples of 512 bytes)
+  static constexpr int kLoop = kBias + kBufs * kKeys * 4;
+  static constexpr int kJoin = WK > 1 ? 4 * 32 * DP * 4 + 4 * 64 * 4 : 0;
+  static constexpr int kLds = kLoop > kJoin ? kLoop : kJoin;
 };
 
-template <class T, int DP, int WR, int WK, int KT>
-__global__ __launch_bounds__(256, sizeof(T) == 4 ? 1 : 2) void att_fwd(Att a) {
-  typedef Tile<T, DP> TL;
+// waves a SIMD that the registers are to leave room for
+template <class T, int DP, int RB>
+constexpr int fwd_waves() { return sizeof(T) == 4 ? 1 : RB * DP > 128 ? 1 : 2; }
+
+template <class T, int DP, int WR, int WK, int KT, int RB>
+__global__ __launch_bounds__(256, (fwd_waves<T, DP, RB>())) void att_fwd(Att a) {
   typedef FwdShape<T, DP, WR, WK, KT> Sh;
-  constexpr int kKeys = Sh::kKeys, NS = DP / 16, ND = DP / 32, NB = KT / 32;
-  extern __shared__ __attribute__((aligned(16))) char lds[];
-  char *kt = lds, *vt = lds + Sh::kTileBytes;
-  float* bias = reinterpret_cast<float*>(lds + 2 * Sh::kTileBytes);
-  const int tid = threadIdx.x, l = tid & 63, w = tid >> 6, h = l >> 5, wr = w % WR, wk = w / WR;
+  constexpr int kKeys = Sh::kKeys, NS = DP / 16, ND = DP / 32, NB = KT / 32, kRows = 32 * WR * RB;
+  constexpr int64_t e = (int64_t)sizeof(T);
+  static_assert(WK == 1 || RB == 1, "the join has one row block a wave");
+  extern __shared__ __attribute__((aligned(1024))) char lds[];
+  const int tid = threadIdx.x, l = tid & 63, w = wave_id(), h = l >> 5, wr = w % WR, wk = w / WR;
   int id = xcd_order(blockIdx.x, gridDim.x);
   const int tile = id % a.tiles;
   id /= a.tiles;
@@ -278,152 +391,188 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? 1 : 2) void att_fwd(Att a) {
   id /= a.splits;
   const int hk = id % a.Hk, c = id / a.Hk;
 
-  const int r = tile * 32 * WR + wr * 32 + (l & 31);
-  int b = 0, i = 0, g = 0;
-  bool live = r < a.R;
-  if (live) {
-    row_of(a, c, r, b, i, g);
-    live = row_live(a, b, i);
-  }
-  const char* qrow = live ? a.q + ((int64_t)b * a.qs[0] + (int64_t)i * a.qs[1] + (int64_t)(hk * a.G + g) * a.qs[2]) * (int64_t)sizeof(T)
-                          : nullptr;
-  typename Ops<T>::Frag qf[NS];
+  const int r0 = tile * kRows + wr * 32 * RB + (l & 31);   // row of block x: r0 + 32 x
+  // a negative scale turns the queries (exact); 0 becomes a scale under which every score rounds to 0
+  const float sc = fmaxf(fabsf(a.scale) * kLog2e, 1e-30f);
+  typename Ops<T>::Frag qf[RB][NS];
+  bool live[RB];
 #pragma unroll
-  for (int s = 0; s < NS; ++s) qf[s] = frag_global<T>(qrow, s, h, a.D);
+  for (int x = 0; x < RB; ++x) {
+    const int r = r0 + 32 * x;
+    int b = 0, i = 0, g = 0;
+    live[x] = r < a.R;
+    if (live[x]) {
+      row_of(a, c, r, b, i, g);
+      live[x] = row_live(a, b, i);
+    }
+    const char* qrow = live[x] ? a.q + ((int64_t)b * a.qs[0] + (int64_t)i * a.qs[1] + (int64_t)(hk * a.G + g) * a.qs[2]) * e : nullptr;
+#pragma unroll
+    for (int s = 0; s < NS; ++s) {
+      qf[x][s] = frag_global<T>(qrow, s, h, a.D);
+      if (a.scale < 0.f) qf[x][s] = -qf[x][s];
+    }
+  }
 
   const int n = key_count(a, c);
   const int nt = (n + kKeys - 1) / kKeys, share = (nt + a.splits - 1) / a.splits;
   const int t0 = min(split * share, nt), t1 = min(t0 + share, nt);
-  const char* kb = a.k + ((int64_t)c * a.ks[0] + (int64_t)hk * a.ks[2]) * (int64_t)sizeof(T);
-  const char* vb = a.v + ((int64_t)c * a.vs[0] + (int64_t)hk * a.vs[2]) * (int64_t)sizeof(T);
   const uint8_t* mask = a.mask ? a.mask + (int64_t)c * a.Lk : nullptr;
   auto allowed = [&](int key) { return key < n && (!mask || mask[key]); };
-
-  f32x16 o[ND];
-#pragma unroll
-  for (int d = 0; d < ND; ++d) o[d] = f32x16{};
-  float m = -kInf, sum = 0.f;
-  const float sc = a.scale * kLog2e;
-
-  Stage<T, DP, kKeys, 256> sk, sv;
-  auto fetch = [&](int t) {
-    const int k0 = t * kKeys;
-    sk.load(tid, a.D, [&](int x) { return allowed(k0 + x) ? kb + (int64_t)(k0 + x) * a.ks[1] * (int64_t)sizeof(T) : nullptr; });
-    sv.load(tid, a.D, [&](int x) { return allowed(k0 + x) ? vb + (int64_t)(k0 + x) * a.vs[1] * (int64_t)sizeof(T) : nullptr; });
+  KeyTile<T, DP, kKeys> kt, vt;
+  kt.init(a.k + ((int64_t)c * a.ks[0] + (int64_t)hk * a.ks[2]) * e, a.ks[1] * e, a.D, tid);
+  vt.init(a.v + ((int64_t)c * a.vs[0] + (int64_t)hk * a.vs[2]) * e, a.vs[1] * e, a.D, tid);
+  auto whole = [&](int t) { return !mask && (t + 1) * kKeys <= n; };
+  const uint32_t lds0 = lds_address(lds);
+  Reader<T, DP> rd;
+  rd.init(lds0, l);
+  float* const biases = reinterpret_cast<float*>(lds + Sh::kBias);
+  auto fetch = [&](int t, int buf) {
+    kt.load(lds0 + buf * Sh::kBuf, t * kKeys, n - t * kKeys, mask != nullptr, allowed);
+    vt.load(lds0 + buf * Sh::kBuf + Sh::kTileBytes, t * kKeys, n - t * kKeys, mask != nullptr, allowed);
+    if (!whole(t) && tid < kKeys) biases[buf * kKeys + tid] = allowed(t * kKeys + tid) ? 0.f : -kInf;
   };
-  if (t0 < t1) fetch(t0);
-  for (int t = t0; t < t1; ++t) {
-    const bool whole = !mask && (t + 1) * kKeys <= n;
-    __syncthreads();
-    sk.store(kt, tid);
-    sv.store(vt, tid);
-    if (!whole && tid < kKeys) bias[tid] = allowed(t * kKeys + tid) ? 0.f : -kInf;
-    __syncthreads();
-    if (t + 1 < t1) fetch(t + 1);
 
-    f32x16 sx[NB];
+  f32x16 o[RB][ND];
+  float m[RB], sum[RB];
 #pragma unroll
-    for (int kb2 = 0; kb2 < NB; ++kb2) {
-      sx[kb2] = f32x16{};
+  for (int x = 0; x < RB; ++x) {
+    m[x] = -kInf, sum[x] = 0.f;
 #pragma unroll
-      for (int s = 0; s < NS; ++s)
-        sx[kb2] = Ops<T>::mma(TL::frag(kt, wk * KT + kb2 * 32 + (l & 31), s, h), qf[s], sx[kb2]);
+    for (int d = 0; d < ND; ++d) o[x][d] = f32x16{};
+  }
+  const float slack = 8.f / sc;   // P may reach 2^8 before the running maximum moves (a rescale of O less often)
+  if (t0 < t1) fetch(t0, 0);
+  auto step = [&](int t, auto which) {
+    constexpr int cur = decltype(which)::value;
+    dma_wait();
+    __syncthreads();   // tile t has landed, and every wave is done with tile t - 1
+    if (Sh::kBufs == 2 && t + 1 < t1) fetch(t + 1, cur ^ 1);
+    const uint32_t kat = cur * Sh::kBuf, vat = kat + Sh::kTileBytes;
+    const float* bias = biases + cur * kKeys;
+    f32x16 sx[RB][NB];
+#pragma unroll
+    for (int kb = 0; kb < NB; ++kb) {
+#pragma unroll
+      for (int x = 0; x < RB; ++x) sx[x][kb] = f32x16{};
+#pragma unroll
+      for (int s = 0; s < NS; ++s) {
+        const auto kf = rd.frag(kat, wk * KT + kb * 32, s);
+#pragma unroll
+        for (int x = 0; x < RB; ++x) sx[x][kb] = Ops<T>::mma(kf, qf[x][s], sx[x][kb]);
+      }
     }
-    float mx = -kInf;
-    if (!whole) {
+    if (!whole(t)) {
 #pragma unroll
-      for (int kb2 = 0; kb2 < NB; ++kb2)
+      for (int kb = 0; kb < NB; ++kb)
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const f32x4 bs = *reinterpret_cast<const f32x4*>(bias + wk * KT + kb2 * 32 + 8 * j + 4 * h);
+          const f32x4 bs = *reinterpret_cast<const f32x4*>(bias + wk * KT + kb * 32 + 8 * j + 4 * h);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) sx[kb2][4 * j + e] = fmaf(sx[kb2][4 * j + e], sc, bs[e]);
+          for (int y = 0; y < 4; ++y)
+#pragma unroll
+            for (int x = 0; x < RB; ++x) sx[x][kb][4 * j + y] += bs[y];
         }
-    } else {
-#pragma unroll
-      for (int kb2 = 0; kb2 < NB; ++kb2)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) sx[kb2][e] *= sc;
     }
 #pragma unroll
-    for (int kb2 = 0; kb2 < NB; ++kb2)
+    for (int x = 0; x < RB; ++x) {
+      float mx = -kInf;
 #pragma unroll
-      for (int e = 0; e < 16; ++e) mx = fmaxf(mx, sx[kb2][e]);
-    mx = max_halves(mx);
-    const float mn = fmaxf(m, mx);
-    const float ref = mn == -kInf ? 0.f : mn;   // nothing allowed yet: exp2(-inf - 0) = 0
-    if (__any(mn > m)) {
-      const float al = __builtin_amdgcn_exp2f(m - ref);
-      sum *= al;
+      for (int kb = 0; kb < NB; ++kb)
 #pragma unroll
-      for (int d = 0; d < ND; ++d)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) o[d][e] *= al;
-      m = mn;
-    }
-#pragma unroll
-    for (int kb2 = 0; kb2 < NB; ++kb2) {
-#pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        sx[kb2][e] = __builtin_amdgcn_exp2f(sx[kb2][e] - ref);
-        sum += sx[kb2][e];
-      }
-#pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        const auto p = to_frag<T>(sx[kb2], s);
+        for (int y = 0; y < 16; ++y) mx = fmaxf(mx, sx[x][kb][y]);
+      mx = max_halves(mx);
+      if (__any(mx > m[x] + slack)) {
+        const float mn = fmaxf(m[x], mx);
+        const float al = __builtin_amdgcn_exp2f((m[x] - (mn == -kInf ? 0.f : mn)) * sc);
+        sum[x] *= al;
 #pragma unroll
         for (int d = 0; d < ND; ++d)
-          o[d] = Ops<T>::mma(TL::frag_t(vt, wk * KT + kb2 * 32 + 16 * s, 32 * d, l), p, o[d]);
+#pragma unroll
+          for (int y = 0; y < 16; ++y) o[x][d][y] *= al;
+        m[x] = mn;
       }
+      const float ref = m[x] == -kInf ? 0.f : -m[x] * sc;   // nothing allowed yet: exp2(-inf) = 0
+#pragma unroll
+      for (int kb = 0; kb < NB; ++kb)
+#pragma unroll
+        for (int y = 0; y < 16; ++y) {
+          sx[x][kb][y] = __builtin_amdgcn_exp2f(fmaf(sx[x][kb][y], sc, ref));
+          sum[x] += sx[x][kb][y];
+        }
     }
-  }
-  sum = sum_halves(sum);
-
-  // ---- join the key waves, normalise, store.  lse in log2 units; an empty row has sum 0: output 0, lse -inf
-  const int64_t grow = ((int64_t)c * a.Hk + hk) * a.R + r;
-  auto put = [&](int rr, bool lv, int bb, int ii, int gg, int d, f32x4 v) {
-    if (!lv) v = f32x4{0.f, 0.f, 0.f, 0.f};   // a row behind its molecule's length
-    if (a.splits > 1) {
-      if (rr < a.R)
-        *reinterpret_cast<f32x4*>(a.part + (((int64_t)split * a.C * a.Hk + (int64_t)c * a.Hk + hk) * a.R + rr) * a.D + d) = v;
-    } else if (rr < a.R) {
-      store4<T>(a.out + ((((int64_t)bb * a.Lq + ii) * a.Hq + hk * a.G + gg) * a.D + d) * (int64_t)sizeof(T), v);
+#pragma unroll
+    for (int kb = 0; kb < NB; ++kb)
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        typename Ops<T>::Frag p[RB];
+#pragma unroll
+        for (int x = 0; x < RB; ++x) p[x] = to_frag<T>(sx[x][kb], s);
+#pragma unroll
+        for (int d = 0; d < ND; ++d) {
+          const auto vf = rd.frag_t(vat, wk * KT + kb * 32 + 16 * s, d);
+#pragma unroll
+          for (int x = 0; x < RB; ++x) o[x][d] = Ops<T>::mma(vf, p[x], o[x][d]);
+        }
+      }
+    if (Sh::kBufs == 1 && t + 1 < t1) {
+      __syncthreads();
+      fetch(t + 1, 0);
     }
   };
+  // the buffer is a constant of each half: every LDS address is a register of the loop plus a constant offset
+  for (int t = t0; t < t1; t += Sh::kBufs) {
+    step(t, Const<0>{});
+    if (Sh::kBufs == 2 && t + 1 < t1) step(t + 1, Const<1>{});
+  }
+
+  // ---- join the key waves, normalise, store.  lse in log2 units; an empty row has sum 0: output 0, lse -inf
+  const int64_t n_rows = (int64_t)a.C * a.Hk * a.R, row0 = ((int64_t)c * a.Hk + hk) * a.R;
+  auto put = [&](int rr, bool lv, int bb, int ii, int gg, int d, f32x4 v) {
+    if (!lv) v = f32x4{0.f, 0.f, 0.f, 0.f};   // a row behind its molecule's length
+    if (a.splits > 1) *reinterpret_cast<f32x4*>(a.part + (split * n_rows + row0 + rr) * a.D + d) = v;
+    else store4<T>(a.out + ((((int64_t)bb * a.Lq + ii) * a.Hq + hk * a.G + gg) * a.D + d) * e, v);
+  };
+  auto put_lse = [&](int rr, bool lv, int bb, int ii, int gg, float mm, float ll) {
+    const float lse = ll == 0.f || !lv ? -kInf : mm * sc + __builtin_amdgcn_logf(ll);
+    if (a.splits > 1) a.part_lse[split * n_rows + row0 + rr] = lse;
+    else if (a.lse) a.lse[((int64_t)bb * a.Hq + hk * a.G + gg) * a.Lq + ii] = lse * kLn2;
+  };
   if constexpr (WK == 1) {
-    const float inv = sum > 0.f ? 1.f / sum : (sum == 0.f ? 0.f : sum);   // NaN stays
-    if (r < a.R) {
+#pragma unroll
+    for (int x = 0; x < RB; ++x) {
+      const int r = r0 + 32 * x;
+      const float tot = sum_halves(sum[x]);
+      const float inv = tot > 0.f ? 1.f / tot : (tot == 0.f ? 0.f : tot);   // NaN stays
+      if (r >= a.R) continue;
+      int b, i, g;
+      row_of(a, c, r, b, i, g);
 #pragma unroll
       for (int d = 0; d < ND; ++d)
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const int dd = 32 * d + 8 * j + 4 * h;
-          if (dd < a.D)
-            put(r, live, b, i, g, dd,
-                f32x4{o[d][4 * j] * inv, o[d][4 * j + 1] * inv, o[d][4 * j + 2] * inv, o[d][4 * j + 3] * inv});
+          const f32x16& y = o[x][d];
+          if (dd < a.D) put(r, live[x], b, i, g, dd, f32x4{y[4 * j] * inv, y[4 * j + 1] * inv, y[4 * j + 2] * inv, y[4 * j + 3] * inv});
         }
-      if (h == 0) {
-        const float lse = sum == 0.f || !live ? -kInf : m + __builtin_amdgcn_logf(sum);
-        if (a.splits > 1) a.part_lse[(int64_t)split * a.C * a.Hk * a.R + grow] = lse;
-        else if (a.lse) a.lse[((int64_t)b * a.Hq + hk * a.G + g) * a.Lq + i] = lse * kLn2;
-      }
+      if (h == 0) put_lse(r, live[x], b, i, g, m[x], tot);
     }
   } else {
     float* jo = reinterpret_cast<float*>(lds);                 // [wave][row][DP], 16-byte chunks swizzled by row
     float* jm = jo + 4 * 32 * DP;                              // [wave][row]
     float* jl = jm + 4 * 32;
+    const float tot = sum_halves(sum[0]);
     __syncthreads();
 #pragma unroll
     for (int d = 0; d < ND; ++d)
 #pragma unroll
       for (int j = 0; j < 4; ++j)
         *reinterpret_cast<f32x4*>(reinterpret_cast<char*>(jo + w * 32 * DP) + Tile<float, DP>::at(l & 31, 8 * d + 2 * j + h)) =
-            f32x4{o[d][4 * j], o[d][4 * j + 1], o[d][4 * j + 2], o[d][4 * j + 3]};
-    if (h == 0) jm[w * 32 + (l & 31)] = m, jl[w * 32 + (l & 31)] = sum;
+            f32x4{o[0][d][4 * j], o[0][d][4 * j + 1], o[0][d][4 * j + 2], o[0][d][4 * j + 3]};
+    if (h == 0) jm[w * 32 + (l & 31)] = m[0], jl[w * 32 + (l & 31)] = tot;
     __syncthreads();
     for (int x = tid; x < WR * 32 * (DP / 4); x += 256) {
       const int ch = x % (DP / 4), row = x / (DP / 4), rw = row >> 5, rl = row & 31;
-      const int rr = tile * 32 * WR + row;
+      const int rr = tile * kRows + row;
       if (rr >= a.R || ch * 4 >= a.D) continue;
       float M = -kInf;
 #pragma unroll
@@ -434,11 +583,11 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? 1 : 2) void att_fwd(Att a) {
 #pragma unroll
       for (int k = 0; k < WK; ++k) {
         const int ww = k * WR + rw;
-        const float e = __builtin_amdgcn_exp2f(jm[ww * 32 + rl] - ref);
-        L += e * jl[ww * 32 + rl];
+        const float f = __builtin_amdgcn_exp2f((jm[ww * 32 + rl] - ref) * sc);
+        L += f * jl[ww * 32 + rl];
         const f32x4 y = *reinterpret_cast<const f32x4*>(reinterpret_cast<const char*>(jo + ww * 32 * DP) + Tile<float, DP>::at(rl, ch));
 #pragma unroll
-        for (int q = 0; q < 4; ++q) v[q] = fmaf(e, y[q], v[q]);
+        for (int q = 0; q < 4; ++q) v[q] = fmaf(f, y[q], v[q]);
       }
       const float inv = L > 0.f ? 1.f / L : (L == 0.f ? 0.f : L);
 #pragma unroll
@@ -447,11 +596,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? 1 : 2) void att_fwd(Att a) {
       row_of(a, c, rr, bb, ii, gg);
       const bool lv = row_live(a, bb, ii);
       put(rr, lv, bb, ii, gg, ch * 4, v);
-      if (ch == 0) {
-        const float lse = L == 0.f || !lv ? -kInf : M + __builtin_amdgcn_logf(L);
-        if (a.splits > 1) a.part_lse[((int64_t)split * a.C * a.Hk + (int64_t)c * a.Hk + hk) * a.R + rr] = lse;
-        else if (a.lse) a.lse[((int64_t)bb * a.Hq + hk * a.G + gg) * a.Lq + ii] = lse * kLn2;
-      }
+      if (ch == 0) put_lse(rr, lv, bb, ii, gg, M, L);
     }
   }
 }
@@ -496,12 +641,9 @@ __global__ __launch_bounds__(256) void att_fwd_join(Att a) {
 // ---------------------------------------------------------------------------------------------------------------
 template <class T, int DP, int WR, int WK, int KT>
 __global__ __launch_bounds__(256, sizeof(T) == 4 ? 1 : 2) void att_dq(Att a) {
-  typedef Tile<T, DP> TL;
   typedef FwdShape<T, DP, WR, WK, KT> Sh;
   constexpr int kKeys = Sh::kKeys, NS = DP / 16, ND = DP / 32, NB = KT / 32;
-  extern __shared__ __attribute__((aligned(16))) char lds[];
-  char *kt = lds, *vt = lds + Sh::kTileBytes;
-  float* bias = reinterpret_cast<float*>(lds + 2 * Sh::kTileBytes);
+  extern __shared__ __attribute__((aligned(1024))) char lds[];
   const int tid = threadIdx.x, l = tid & 63, w = tid >> 6, h = l >> 5, wr = w % WR, wk = w / WR;
   int id = xcd_order(blockIdx.x, gridDim.x);
   const int tile = id % a.tiles;
@@ -533,7 +675,8 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? 1 : 2) void att_dq(Att a) {
     for (int x = 0; x < 8; ++x) delta = fmaf((float)df[s][x], (float)of[x], delta);
   }
   delta = sum_halves(delta);
-  const float sc = a.scale * kLog2e;
+  // (a scale of 0 would make NaN of a masked key's -inf)
+  const float sc = a.scale == 0.f ? 1e-30f : a.scale * kLog2e, sg = a.scale < 0.f ? -1.f : 1.f;
   float lse = kInf;
   if (live) {
     lse = a.lse[((int64_t)b * a.Hq + hq) * a.Lq + i] * kLog2e;
@@ -548,55 +691,72 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? 1 : 2) void att_dq(Att a) {
   const int n = key_count(a, c);
   const int nt = (n + kKeys - 1) / kKeys, share = (nt + a.splits - 1) / a.splits;
   const int t0 = min(split * share, nt), t1 = min(t0 + share, nt);
-  const char* kb = a.k + ((int64_t)c * a.ks[0] + (int64_t)hk * a.ks[2]) * e;
-  const char* vb = a.v + ((int64_t)c * a.vs[0] + (int64_t)hk * a.vs[2]) * e;
   const uint8_t* mask = a.mask ? a.mask + (int64_t)c * a.Lk : nullptr;
   auto allowed = [&](int key) { return key < n && (!mask || mask[key]); };
+  KeyTile<T, DP, kKeys> kt, vt;
+  kt.init(a.k + ((int64_t)c * a.ks[0] + (int64_t)hk * a.ks[2]) * e, a.ks[1] * e, a.D, tid);
+  vt.init(a.v + ((int64_t)c * a.vs[0] + (int64_t)hk * a.vs[2]) * e, a.vs[1] * e, a.D, tid);
+  auto whole = [&](int t) { return !mask && (t + 1) * kKeys <= n; };
+  const uint32_t lds0 = lds_address(lds);
+  Reader<T, DP> rd;
+  rd.init(lds0, l);
+  float* const biases = reinterpret_cast<float*>(lds + Sh::kBias);
+  auto fetch = [&](int t, int buf) {
+    kt.load(lds0 + buf * Sh::kBuf, t * kKeys, n - t * kKeys, mask != nullptr, allowed);
+    vt.load(lds0 + buf * Sh::kBuf + Sh::kTileBytes, t * kKeys, n - t * kKeys, mask != nullptr, allowed);
+    if (!whole(t) && tid < kKeys) biases[buf * kKeys + tid] = allowed(t * kKeys + tid) ? 0.f : -kInf;
+  };
 
   f32x16 acc[ND];
 #pragma unroll
   for (int d = 0; d < ND; ++d) acc[d] = f32x16{};
-  Stage<T, DP, kKeys, 256> sk, sv;
-  auto fetch = [&](int t) {
-    const int k0 = t * kKeys;
-    sk.load(tid, a.D, [&](int x) { return allowed(k0 + x) ? kb + (int64_t)(k0 + x) * a.ks[1] * e : nullptr; });
-    sv.load(tid, a.D, [&](int x) { return allowed(k0 + x) ? vb + (int64_t)(k0 + x) * a.vs[1] * e : nullptr; });
-  };
-  if (t0 < t1) fetch(t0);
-  for (int t = t0; t < t1; ++t) {
-    const bool whole = !mask && (t + 1) * kKeys <= n;
-    __syncthreads();
-    sk.store(kt, tid);
-    sv.store(vt, tid);
-    if (!whole && tid < kKeys) bias[tid] = allowed(t * kKeys + tid) ? 0.f : -kInf;
-    __syncthreads();
-    if (t + 1 < t1) fetch(t + 1);
+  if (t0 < t1) fetch(t0, 0);
+  auto step = [&](int t, auto which) {
+    constexpr int cur = decltype(which)::value;
+    dma_wait();
+    __syncthreads();   // tile t has landed, and every wave is done with tile t - 1
+    if (Sh::kBufs == 2 && t + 1 < t1) fetch(t + 1, cur ^ 1);
+    const uint32_t kat = cur * Sh::kBuf, vat = kat + Sh::kTileBytes;
+    const float* bias = biases + cur * kKeys;
+    const bool all = whole(t);
 #pragma unroll
-    for (int kb2 = 0; kb2 < NB; ++kb2) {
-      const int k0 = wk * KT + kb2 * 32;
+    for (int kb = 0; kb < NB; ++kb) {
+      const int k0 = wk * KT + kb * 32;
       f32x16 sx = f32x16{}, dp = f32x16{};
 #pragma unroll
       for (int s = 0; s < NS; ++s) {
-        sx = Ops<T>::mma(TL::frag(kt, k0 + (l & 31), s, h), qf[s], sx);
-        dp = Ops<T>::mma(TL::frag(vt, k0 + (l & 31), s, h), df[s], dp);
+        sx = Ops<T>::mma(rd.frag(kat, k0, s), qf[s], sx);
+        dp = Ops<T>::mma(rd.frag(vat, k0, s), df[s], dp);
+      }
+      if (!all) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const f32x4 bs = *reinterpret_cast<const f32x4*>(bias + k0 + 8 * j + 4 * h);
+#pragma unroll
+          for (int x = 0; x < 4; ++x) sx[4 * j + x] = bs[x] < 0.f ? bs[x] * sg : sx[4 * j + x];
+        }
       }
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        f32x4 bs = {0.f, 0.f, 0.f, 0.f};
-        if (!whole) bs = *reinterpret_cast<const f32x4*>(bias + k0 + 8 * j + 4 * h);
-#pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          const float p = __builtin_amdgcn_exp2f(fmaf(sx[4 * j + x], sc, bs[x] - lse));
-          sx[4 * j + x] = p * (dp[4 * j + x] - delta);
-        }
+      for (int x = 0; x < 16; ++x) {
+        const float p = __builtin_amdgcn_exp2f(fmaf(sx[x], sc, -lse));
+        sx[x] = p * (dp[x] - delta);
       }
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
         const auto dsf = to_frag<T>(sx, s);
 #pragma unroll
-        for (int d = 0; d < ND; ++d) acc[d] = Ops<T>::mma(TL::frag_t(kt, k0 + 16 * s, 32 * d, l), dsf, acc[d]);
+        for (int d = 0; d < ND; ++d) acc[d] = Ops<T>::mma(rd.frag_t(kat, k0 + 16 * s, d), dsf, acc[d]);
       }
     }
+    if (Sh::kBufs == 1 && t + 1 < t1) {
+      __syncthreads();
+      fetch(t + 1, 0);
+    }
+  };
+  // the buffer is a constant of each half: every LDS address is a register of the loop plus a constant offset
+  for (int t = t0; t < t1; t += Sh::kBufs) {
+    step(t, Const<0>{});
+    if (Sh::kBufs == 2 && t + 1 < t1) step(t + 1, Const<1>{});
   }
 
   const int64_t n_rows = (int64_t)a.C * a.Hk * a.R, row0 = ((int64_t)c * a.Hk + hk) * a.R;
@@ -649,24 +809,29 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? 1 : 2) void att_dq(Att a) {
 // ---------------------------------------------------------------------------------------------------------------
 template <class T, int DP, int WY, int WX>
 struct DkvShape {
-  static constexpr int kRows = 32 * WX;
+  // V of the workgroup's keys: registers (a B operand a wave), or LDS where those would leave none to read ahead with
+  static constexpr bool kVLds = DP == 128;
+  static constexpr int kVBytes = kVLds ? 32 * WY * DP * (int)sizeof(T) : 0;
+  // row blocks a wave takes of a tile: 2 where the registers allow (half the barriers; a tile is whole chunks)
+  static constexpr int kXB = DP * (int)sizeof(T) <= 128 ? 2 : 1;
+  static constexpr int kRows = 32 * WX * kXB;
   static constexpr int kTileBytes = kRows * DP * (int)sizeof(T);
-  static constexpr int kLoop = 2 * kTileBytes + 2 * kRows * 4;
+  static constexpr int kBuf = 2 * kTileBytes;   // Q, dO
+  static constexpr int kBufs = 2 * (kBuf + kRows * 8) + kVBytes <= 160 * 1024 ? 2 : 1;
+  static constexpr int kV = kBufs * kBuf;       // behind the tiles: V, then the rows' lse and delta
+  static constexpr int kStat = kV + kVBytes;
+  static constexpr int kLoop = kStat + kBufs * kRows * 8;
   static constexpr int kJoin = WX > 1 ? 4 * 32 * DP * 4 : 0;
   static constexpr int kLds = kLoop > kJoin ? kLoop : kJoin;
 };
 
 template <class T, int DP, int WY, int WX>
-__global__ __launch_bounds__(256, 1) void att_dkv(Att a) {
-  typedef Tile<T, DP> TL;
+__global__ __launch_bounds__(256, sizeof(T) == 4 ? 1 : 2) void att_dkv(Att a) {
   typedef DkvShape<T, DP, WY, WX> Sh;
   constexpr int kRows = Sh::kRows, NS = DP / 16, ND = DP / 32;
   constexpr int64_t e = (int64_t)sizeof(T);
-  extern __shared__ __attribute__((aligned(16))) char lds[];
-  char *qt = lds, *dt = lds + Sh::kTileBytes;
-  float* rl = reinterpret_cast<float*>(lds + 2 * Sh::kTileBytes);
-  float* rd = rl + kRows;
-  const int tid = threadIdx.x, l = tid & 63, w = tid >> 6, h = l >> 5, wy = w % WY, wx = w / WY;
+  extern __shared__ __attribute__((aligned(1024))) char lds[];
+  const int tid = threadIdx.x, l = tid & 63, w = wave_id(), h = l >> 5, wy = w % WY, wx = w / WY;
   int id = xcd_order(blockIdx.x, gridDim.x);
   const int tile = id % a.tiles;
   id /= a.tiles;
@@ -680,9 +845,28 @@ __global__ __launch_bounds__(256, 1) void att_dkv(Att a) {
   const bool ok = key < n && (!mask || mask[key]);
   const char* krow = ok ? a.k + ((int64_t)c * a.ks[0] + (int64_t)key * a.ks[1] + (int64_t)hk * a.ks[2]) * e : nullptr;
   const char* vrow = ok ? a.v + ((int64_t)c * a.vs[0] + (int64_t)key * a.vs[1] + (int64_t)hk * a.vs[2]) * e : nullptr;
-  typename Ops<T>::Frag kf[NS], vf[NS];
+  const uint32_t lds0 = lds_address(lds);
+  Reader<T, DP> rdr;
+  rdr.init(lds0, l);
+  typename Ops<T>::Frag kf[NS], vf[Sh::kVLds ? 1 : NS];
 #pragma unroll
-  for (int s = 0; s < NS; ++s) kf[s] = frag_global<T>(krow, s, h, a.D), vf[s] = frag_global<T>(vrow, s, h, a.D);
+  for (int s = 0; s < NS; ++s) {
+    kf[s] = frag_global<T>(krow, s, h, a.D);
+    const auto x = frag_global<T>(vrow, s, h, a.D);
+    if constexpr (Sh::kVLds) {
+      // a key's row belongs to the wave that reads it; the row waves (WX) of a key block write the same values
+      char* p = lds + Sh::kV;
+      const int r = wy * 32 + (l & 31);
+      if constexpr (sizeof(T) == 2) {
+        *reinterpret_cast<typename Ops<T>::Frag*>(p + Tile<T, DP>::at(r, 2 * s + h)) = x;
+      } else {
+        *reinterpret_cast<f32x4*>(p + Tile<T, DP>::at(r, 4 * s + 2 * h)) = f32x4{x[0], x[1], x[2], x[3]};
+        *reinterpret_cast<f32x4*>(p + Tile<T, DP>::at(r, 4 * s + 2 * h + 1)) = f32x4{x[4], x[5], x[6], x[7]};
+      }
+    } else {
+      vf[s] = x;
+    }
+  }
   f32x16 dk[ND], dv[ND];
 #pragma unroll
   for (int d = 0; d < ND; ++d) dk[d] = f32x16{}, dv[d] = f32x16{};
@@ -693,65 +877,76 @@ __global__ __launch_bounds__(256, 1) void att_dkv(Att a) {
   const int64_t row0 = ((int64_t)c * a.Hk + hk) * a.R;
   const float sc = a.scale * kLog2e;
 
-  Stage<T, DP, kRows, 256> sq, sd;
+  float* const stats = reinterpret_cast<float*>(lds + Sh::kStat);
+  const bool fast = a.flat && !a.qlen && kRows % a.G == 0;
+  RowTile<T, DP, kRows> tq, td;
+  tq.init(a, a.q, a.qs, c, hk, tid, fast);
+  td.init(a, a.dout, a.ds, c, hk, tid, fast);
   float nl = kInf, nd = 0.f;
-  auto fetch = [&](int t) {
+  auto fetch = [&](int t, int buf) {
     const int r0 = t * kRows;
-    sq.load(tid, a.D, [&](int x) -> const char* {
-      if (r0 + x >= a.R) return nullptr;
-      int b, i, g;
-      row_of(a, c, r0 + x, b, i, g);
-      if (!row_live(a, b, i)) return nullptr;
-      return a.q + ((int64_t)b * a.qs[0] + (int64_t)i * a.qs[1] + (int64_t)(hk * a.G + g) * a.qs[2]) * e;
-    });
-    sd.load(tid, a.D, [&](int x) -> const char* {
-      if (r0 + x >= a.R) return nullptr;
-      int b, i, g;
-      row_of(a, c, r0 + x, b, i, g);
-      if (!row_live(a, b, i)) return nullptr;
-      return a.dout + ((int64_t)b * a.ds[0] + (int64_t)i * a.ds[1] + (int64_t)(hk * a.G + g) * a.ds[2]) * e;
-    });
+    tq.load(a, lds0 + buf * Sh::kBuf, c, r0, tid, fast);
+    td.load(a, lds0 + buf * Sh::kBuf + Sh::kTileBytes, c, r0, tid, fast);
     if (tid < kRows) {
       const bool in = r0 + tid < a.R;
       nl = in ? a.row_lse[row0 + r0 + tid] : kInf;
       nd = in ? a.row_delta[row0 + r0 + tid] : 0.f;
     }
   };
-  if (t0 < t1) fetch(t0);
+  auto publish = [&](int buf) {
+    if (tid < kRows) stats[buf * 2 * kRows + tid] = nl, stats[(buf * 2 + 1) * kRows + tid] = nd;
+  };
+  if (t0 < t1) {
+    fetch(t0, 0);
+    publish(0);
+  }
   for (int t = t0; t < t1; ++t) {
-    __syncthreads();
-    sq.store(qt, tid);
-    sd.store(dt, tid);
-    if (tid < kRows) rl[tid] = nl, rd[tid] = nd;
-    __syncthreads();
-    if (t + 1 < t1) fetch(t + 1);
-    const int x0 = wx * 32;
-    f32x16 sx = f32x16{}, dp = f32x16{};
+    const int cur = Sh::kBufs == 2 ? (t - t0) & 1 : 0, next = Sh::kBufs == 2 ? cur ^ 1 : 0;
+    dma_wait();
+    __syncthreads();   // tile t has landed, and every wave is done with tile t - 1
+    if (Sh::kBufs == 2 && t + 1 < t1) fetch(t + 1, next);
+    const uint32_t qat = cur * Sh::kBuf, dat = qat + Sh::kTileBytes;
+    const float* rl = stats + cur * 2 * kRows;
+    const float* rd = rl + kRows;
 #pragma unroll
-    for (int s = 0; s < NS; ++s) {
-      sx = Ops<T>::mma(TL::frag(qt, x0 + (l & 31), s, h), kf[s], sx);
-      dp = Ops<T>::mma(TL::frag(dt, x0 + (l & 31), s, h), vf[s], dp);
-    }
+    for (int xb = 0; xb < Sh::kXB; ++xb) {
+      const int x0 = (wx * Sh::kXB + xb) * 32;
+      if (xb > 0 && t * kRows + x0 >= a.R) break;
+      f32x16 sx = f32x16{}, dp = f32x16{};
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const f32x4 ls = *reinterpret_cast<const f32x4*>(rl + x0 + 8 * j + 4 * h);
-      const f32x4 de = *reinterpret_cast<const f32x4*>(rd + x0 + 8 * j + 4 * h);
+      for (int s = 0; s < NS; ++s) {
+        sx = Ops<T>::mma(rdr.frag(qat, x0, s), kf[s], sx);
+        if constexpr (Sh::kVLds) dp = Ops<T>::mma(rdr.frag(dat, x0, s), rdr.frag(Sh::kV, wy * 32, s), dp);
+        else dp = Ops<T>::mma(rdr.frag(dat, x0, s), vf[s], dp);
+      }
 #pragma unroll
-      for (int x = 0; x < 4; ++x) {
-        float p = __builtin_amdgcn_exp2f(fmaf(sx[4 * j + x], sc, -ls[x]));
-        p = ok ? p : 0.f;
-        sx[4 * j + x] = p;
-        dp[4 * j + x] = p * (dp[4 * j + x] - de[x]);
+      for (int j = 0; j < 4; ++j) {
+        const f32x4 ls = *reinterpret_cast<const f32x4*>(rl + x0 + 8 * j + 4 * h);
+        const f32x4 de = *reinterpret_cast<const f32x4*>(rd + x0 + 8 * j + 4 * h);
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          float p = __builtin_amdgcn_exp2f(fmaf(sx[4 * j + x], sc, -ls[x]));
+          p = ok ? p : 0.f;
+          sx[4 * j + x] = p;
+          dp[4 * j + x] = p * (dp[4 * j + x] - de[x]);
+        }
+      }
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        const auto pf = to_frag<T>(sx, s), sf = to_frag<T>(dp, s);
+#pragma unroll
+        for (int d = 0; d < ND; ++d) {
+          dv[d] = Ops<T>::mma(rdr.frag_t(dat, x0 + 16 * s, d), pf, dv[d]);
+          dk[d] = Ops<T>::mma(rdr.frag_t(qat, x0 + 16 * s, d), sf, dk[d]);
+        }
       }
     }
-#pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      const auto pf = to_frag<T>(sx, s), sf = to_frag<T>(dp, s);
-#pragma unroll
-      for (int d = 0; d < ND; ++d) {
-        dv[d] = Ops<T>::mma(TL::frag_t(dt, x0 + 16 * s, 32 * d, l), pf, dv[d]);
-        dk[d] = Ops<T>::mma(TL::frag_t(qt, x0 + 16 * s, 32 * d, l), sf, dk[d]);
+    if (t + 1 < t1) {
+      if (Sh::kBufs == 1) {
+        __syncthreads();
+        fetch(t + 1, next);
       }
+      publish(next);
     }
   }
 

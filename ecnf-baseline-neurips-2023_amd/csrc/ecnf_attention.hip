@@ -39,8 +39,8 @@ template <int DP>
 hipError_t fwd(const Att& in, hipStream_t s) {
   const Plan p = plan_fwd(in);
   const Att a = with_plan(in, p, in.part);
-  hipError_t e = p.narrow ? launch(att_fwd<T, DP, 1, 4, 32>, p.grid, FwdShape<T, DP, 1, 4, 32>::kLds, a, s)
-                          : launch(att_fwd<T, DP, 4, 1, 64>, p.grid, FwdShape<T, DP, 4, 1, 64>::kLds, a, s);
+  hipError_t e = p.narrow ? launch(att_fwd<T, DP, 1, 4, 32, 1>, p.grid, FwdShape<T, DP, 1, 4, 32>::kLds, a, s)
+                          : launch(att_fwd<T, DP, 4, 1, 64, 1>, p.grid, FwdShape<T, DP, 4, 1, 64>::kLds, a, s);
   if (e != hipSuccess || p.splits == 1) return e;
   const int64_t n = (int64_t)a.C * a.Hk * a.R * (a.D / 4);
   att_fwd_join<T><<<dim3((unsigned)((n + 255) / 256)), dim3(256), 0, s>>>(a);

@@ -447,8 +447,18 @@ int build_att(const ecnf_attention* o, int what, Att* a, bool pointers) {
     a->qs[d] = o->q_stride[d], a->ks[d] = o->k_stride[d], a->vs[d] = o->v_stride[d], a->ds[d] = o->out_grad_stride[d];
   a->dG = fast_div((uint32_t)G);
   a->dL = fast_div((uint32_t)(o->n_queries ? o->n_queries : 1));
-  if (!pointers) return ECNF_OK;
   const int e = elem_size(o->dtype);
+  // tiles of keys are addressed with 32-bit offsets from their first row, tiles of query rows (at most 256) too where
+  // the tokens of a context are evenly spaced
+  auto span = [&](const int64_t* st, int d) { return st[d] * e * 256 < (1ll << 31); };
+  if (o->context_length > 1 && (!span(o->k_stride, 1) || !span(o->v_stride, 1)))
+    return fail(ECNF_E_UNSUPPORTED, "rows of k and v must be less than 8 MiB apart");
+  auto even = [&](const int64_t* st) {
+    return (per <= 1 || o->n_queries <= 1 || st[0] == st[1] * o->n_queries) && span(st, 1) && span(st, 2);
+  };
+  if (o->n_queries == 1) a->qs[1] = a->qs[0], a->ds[1] = a->ds[0];   // one token a molecule: its stride is the batch's
+  a->flat = even(a->qs) && (!what || even(a->ds));
+  if (!pointers) return ECNF_OK;
   const bool rows = a->R > 0, keys = a->Lk > 0;
   if ((rows && (!o->q || !o->out)) || (keys && (!o->k || !o->v))) return fail(ECNF_E_INVALID, "NULL argument");
   if (what && ((rows && (!o->out_grad || !o->q_grad || !o->lse)) || (keys && (!o->k_grad || !o->v_grad))))
