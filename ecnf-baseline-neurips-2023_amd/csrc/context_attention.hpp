@@ -440,6 +440,7 @@ __global__ __launch_bounds__(256, (fwd_waves<T, DP, RB>())) void att_fwd(Att a) 
 #pragma unroll
     for (int d = 0; d < ND; ++d) o[x][d] = f32x16{};
   }
+  const bool idle = tile * kRows + wr * 32 * RB >= a.R;
   const float slack = 8.f / sc;   // P may reach 2^8 before the running maximum moves (a rescale of O less often)
   if (t0 < t1) fetch(t0, 0);
   auto step = [&](int t, auto which) {
@@ -449,6 +450,7 @@ __global__ __launch_bounds__(256, (fwd_waves<T, DP, RB>())) void att_fwd(Att a) 
     if (Sh::kBufs == 2 && t + 1 < t1) fetch(t + 1, cur ^ 1);
     const uint32_t kat = cur * Sh::kBuf, vat = kat + Sh::kTileBytes;
     const float* bias = biases + cur * kKeys;
+    if (!idle && (WK == 1 || t * kKeys + wk * KT < n)) {   // the wave has rows, and keys of this tile
     f32x16 sx[RB][NB];
 #pragma unroll
     for (int kb = 0; kb < NB; ++kb) {
@@ -514,6 +516,7 @@ __global__ __launch_bounds__(256, (fwd_waves<T, DP, RB>())) void att_fwd(Att a) 
           for (int x = 0; x < RB; ++x) o[x][d] = Ops<T>::mma(vf, p[x], o[x][d]);
         }
       }
+    }
     if (Sh::kBufs == 1 && t + 1 < t1) {
       __syncthreads();
       fetch(t + 1, 0);
@@ -707,6 +710,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? 1 : 2) void att_dq(Att a) {
     if (!whole(t) && tid < kKeys) biases[buf * kKeys + tid] = allowed(t * kKeys + tid) ? 0.f : -kInf;
   };
 
+  const bool idle = tile * 32 * WR + wr * 32 >= a.R;
   f32x16 acc[ND];
 #pragma unroll
   for (int d = 0; d < ND; ++d) acc[d] = f32x16{};
@@ -719,9 +723,11 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? 1 : 2) void att_dq(Att a) {
     const uint32_t kat = cur * Sh::kBuf, vat = kat + Sh::kTileBytes;
     const float* bias = biases + cur * kKeys;
     const bool all = whole(t);
+    if (!idle)
 #pragma unroll
     for (int kb = 0; kb < NB; ++kb) {
       const int k0 = wk * KT + kb * 32;
+      if (t * kKeys + k0 >= n) break;
       f32x16 sx = f32x16{}, dp = f32x16{};
 #pragma unroll
       for (int s = 0; s < NS; ++s) {
@@ -878,6 +884,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? 1 : 2) void att_dkv(Att a) {
   const float sc = a.scale * kLog2e;
 
   float* const stats = reinterpret_cast<float*>(lds + Sh::kStat);
+  const bool idle = (tile * WY + wy) * 32 >= n;
   const bool fast = a.flat && !a.qlen && kRows % a.G == 0;
   RowTile<T, DP, kRows> tq, td;
   tq.init(a, a.q, a.qs, c, hk, tid, fast);
@@ -908,10 +915,11 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? 1 : 2) void att_dkv(Att a) {
     const uint32_t qat = cur * Sh::kBuf, dat = qat + Sh::kTileBytes;
     const float* rl = stats + cur * 2 * kRows;
     const float* rd = rl + kRows;
+    if (!idle)
 #pragma unroll
     for (int xb = 0; xb < Sh::kXB; ++xb) {
       const int x0 = (wx * Sh::kXB + xb) * 32;
-      if (xb > 0 && t * kRows + x0 >= a.R) break;
+      if (t * kRows + x0 >= a.R) break;
       f32x16 sx = f32x16{}, dp = f32x16{};
 #pragma unroll
       for (int s = 0; s < NS; ++s) {

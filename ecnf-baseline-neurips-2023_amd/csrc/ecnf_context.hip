@@ -128,6 +128,7 @@ __device__ __forceinline__ int axis_of(const Norm& a, int pair) {   // n_axes: n
 
 template <class T, int VE, bool GRAD>
 __global__ __launch_bounds__(256) void qk_norm_kernel(Norm a) {
+  constexpr int U = GRAD ? 1 : 2;
   __shared__ float2 cs[kCsEntries];
   __shared__ float red[GRAD ? 256 * 2 * VE : 1];
   const int tid = threadIdx.x;
@@ -168,56 +169,66 @@ __global__ __launch_bounds__(256) void qk_norm_kernel(Norm a) {
     }
     __syncthreads();
     const int rows = nt * s.H;
-    for (int rs = slot; rs < rows; rs += slots) {
-      const int tt = (int)s.dH.div(rs), head = rs - tt * s.H, tok = tok0 + tt;
-      const int b = (int)s.dL.div(tok), i = tok - b * s.L;
-      float xa[VE], xb[VE], ya[VE], yb[VE], ss = 0.f, dot = 0.f;
+    for (int rs = slot; rs < rows; rs += U * slots) {
+      // U rows at once: their loads are in flight together
+      float xa[U][VE], xb[U][VE], da[U][VE], db[U][VE];
+      int tt[U], head[U];
 #pragma unroll
-      for (int q = 0; q < VE; ++q) xa[q] = xb[q] = ya[q] = yb[q] = 0.f;
-      if (on) {
-        load_pairs<T, VE>(s.x + ((int64_t)b * s.xs[0] + (int64_t)i * s.xs[1] + (int64_t)head * s.xs[2]) * (int64_t)sizeof(T), inter, lo, hi, xa, xb);
-        if (GRAD) {
-          float da[VE], db[VE];
-          load_pairs<T, VE>(s.dy + ((int64_t)b * s.gs[0] + (int64_t)i * s.gs[1] + (int64_t)head * s.gs[2]) * (int64_t)sizeof(T), inter, lo, hi, da, db);
+      for (int u = 0; u < U; ++u) {
+        const int rr = min(rs + u * slots, rows - 1);   // behind the last row: read again, not written
+        tt[u] = (int)s.dH.div(rr);
+        head[u] = rr - tt[u] * s.H;
+        const int tok = tok0 + tt[u], b = (int)s.dL.div(tok), i = tok - b * s.L;
+        if (on) {
+          load_pairs<T, VE>(s.x + ((int64_t)b * s.xs[0] + (int64_t)i * s.xs[1] + (int64_t)head[u] * s.xs[2]) * (int64_t)sizeof(T), inter, lo, hi, xa[u], xb[u]);
+          if (GRAD)
+            load_pairs<T, VE>(s.dy + ((int64_t)b * s.gs[0] + (int64_t)i * s.gs[1] + (int64_t)head[u] * s.gs[2]) * (int64_t)sizeof(T), inter, lo, hi, da[u], db[u]);
+        } else {
 #pragma unroll
-          for (int q = 0; q < VE; ++q) {
-            const float2 t = cs[tt * a.half + p0 + q];
-            ya[q] = fmaf(da[q], t.x, db[q] * t.y);
-            yb[q] = fmaf(db[q], t.x, -(da[q] * t.y));
+          for (int q = 0; q < VE; ++q) xa[u][q] = xb[u][q] = da[u][q] = db[u][q] = 0.f;
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        float2 t[VE];
+#pragma unroll
+        for (int q = 0; q < VE; ++q) t[q] = on ? cs[tt[u] * a.half + p0 + q] : make_float2(1.f, 0.f);
+        float ya[VE], yb[VE], ss = 0.f, dot = 0.f;
+#pragma unroll
+        for (int q = 0; q < VE; ++q) {
+          ss = fmaf(xa[u][q], xa[u][q], fmaf(xb[u][q], xb[u][q], ss));
+          if (GRAD) {
+            ya[q] = fmaf(da[u][q], t[q].x, db[u][q] * t[q].y);
+            yb[q] = fmaf(db[u][q], t[q].x, -(da[u][q] * t[q].y));
+            dot = fmaf(ya[q] * wa[q], xa[u][q], fmaf(yb[q] * wb[q], xb[u][q], dot));
           }
         }
-      }
-#pragma unroll
-      for (int q = 0; q < VE; ++q) {
-        ss = fmaf(xa[q], xa[q], fmaf(xb[q], xb[q], ss));
-        if (GRAD) dot = fmaf(ya[q] * wa[q], xa[q], fmaf(yb[q] * wb[q], xb[q], dot));
-      }
-      for (int m = a.lp >> 1; m; m >>= 1) {
-        ss += __shfl_xor(ss, m);
-        if (GRAD) dot += __shfl_xor(dot, m);
-      }
-      const float r = 1.f / sqrtf(ss / (float)a.D + a.eps);
-      if (!on) continue;
-      char* o = s.out + ((int64_t)tok * s.H + head) * a.D * (int64_t)sizeof(T);
-      if constexpr (GRAD) {
-        const float m = r * r * (dot / (float)a.D);
-#pragma unroll
-        for (int q = 0; q < VE; ++q) {
-          ga[q] = fmaf(ya[q], xa[q] * r, ga[q]);
-          gb[q] = fmaf(yb[q], xb[q] * r, gb[q]);
-          ya[q] = r * (ya[q] * wa[q] - xa[q] * m);
-          yb[q] = r * (yb[q] * wb[q] - xb[q] * m);
+        for (int m = a.lp >> 1; m; m >>= 1) {
+          ss += __shfl_xor(ss, m);
+          if (GRAD) dot += __shfl_xor(dot, m);
         }
-      } else {
+        const float r = 1.f / sqrtf(ss / (float)a.D + a.eps);
+        if (!on || rs + u * slots >= rows) continue;
+        char* o = s.out + ((int64_t)(tok0 + tt[u]) * s.H + head[u]) * a.D * (int64_t)sizeof(T);
+        if constexpr (GRAD) {
+          const float m = r * r * (dot / (float)a.D);
 #pragma unroll
-        for (int q = 0; q < VE; ++q) {
-          const float2 t = cs[tt * a.half + p0 + q];
-          const float u = xa[q] * r * wa[q], v = xb[q] * r * wb[q];
-          ya[q] = fmaf(u, t.x, -(v * t.y));
-          yb[q] = fmaf(u, t.y, v * t.x);
+          for (int q = 0; q < VE; ++q) {
+            ga[q] = fmaf(ya[q], xa[u][q] * r, ga[q]);
+            gb[q] = fmaf(yb[q], xb[u][q] * r, gb[q]);
+            ya[q] = r * (ya[q] * wa[q] - xa[u][q] * m);
+            yb[q] = r * (yb[q] * wb[q] - xb[u][q] * m);
+          }
+        } else {
+#pragma unroll
+          for (int q = 0; q < VE; ++q) {
+            const float x = xa[u][q] * r * wa[q], y = xb[u][q] * r * wb[q];
+            ya[q] = fmaf(x, t[q].x, -(y * t[q].y));
+            yb[q] = fmaf(x, t[q].y, y * t[q].x);
+          }
         }
+        store_pairs<T, VE>(o, inter, lo, hi, ya, yb);
       }
-      store_pairs<T, VE>(o, inter, lo, hi, ya, yb);
     }
   }
   if constexpr (GRAD) {
@@ -242,23 +253,32 @@ __global__ __launch_bounds__(256) void qk_norm_kernel(Norm a) {
   }
 }
 
-// weight gradients: the blocks' partials summed in a fixed order; blockIdx.y: 0 q, 1 k; 16 columns x 16 lanes a block
-__global__ __launch_bounds__(256) void qk_norm_dw_kernel(Norm a) {
-  __shared__ float red[16][17];
+// weight gradients: the blocks' partials summed in a fixed order; blockIdx.y: 0 q, 1 k; 16 columns x 64 lanes a block,
+// so that a lane's few loads are in flight together
+__global__ __launch_bounds__(1024) void qk_norm_dw_kernel(Norm a) {
+  __shared__ float red[64][17];
   const NormSide& s = a.s[blockIdx.y];
   if (!s.dw) return;
-  const int d = blockIdx.x * 16 + (threadIdx.x & 15), y = threadIdx.x >> 4;
+  const int x = threadIdx.x & 15, d = blockIdx.x * 16 + x, y = threadIdx.x >> 4;
   const float* p = a.part + (blockIdx.y ? (int64_t)a.s[0].blocks * a.D : 0);
   float v = 0.f;
-  if (d < a.D)
-    for (int b = y; b < s.blocks; b += 16) v += p[(int64_t)b * a.D + d];
-  red[y][threadIdx.x & 15] = v;
-  __syncthreads();
-  if (y == 0 && d < a.D) {
-    float t = 0.f;
-    for (int k = 0; k < 16; ++k) t += red[k][threadIdx.x];
-    s.dw[d] = t;
+  if (d < a.D) {
+#pragma unroll
+    for (int k = 0; k < kMaxGradBlocks / 64; ++k) {
+      const int b = y + 64 * k;
+      if (b < s.blocks) v += p[(int64_t)b * a.D + d];
+    }
   }
+  red[y][x] = v;
+  __syncthreads();
+  if (y < 4) {
+    float t = 0.f;
+#pragma unroll
+    for (int k = 0; k < 16; ++k) t += red[16 * y + k][x];
+    red[16 * y][x] = t;   // row 16 y is this lane's own
+  }
+  __syncthreads();
+  if (y == 0 && d < a.D) s.dw[d] = (red[0][x] + red[16][x]) + (red[32][x] + red[48][x]);
 }
 
 // ---------------------------------------------------------------------------------------------------------------
@@ -326,7 +346,10 @@ int build_norm(const ecnf_qk_norm* o, bool grad, Norm* a, int* ve, bool pointers
   for (int x = 0; x < o->n_axes; ++x) {
     const int d = o->axes[x];
     if (d < 2 || d % 2 || at + d / 2 > a->half) return fail(ECNF_E_INVALID, "axes must be even, >= 2 and sum to at most head_dim");
-    for (int j = 0; j < d / 2; ++j) a->turns[at + j] = std::pow(o->theta, -2.0 * j / d) / 6.283185307179586476925286766559;
+    // theta^(-2j/d) as powers of theta^(-2/d): in extended precision their error stays below a step of a double
+    const long double ratio = std::pow((long double)o->theta, -2.0L / d);
+    long double power = 1.0L / 6.283185307179586476925286766559L;
+    for (int j = 0; j < d / 2; ++j, power *= ratio) a->turns[at + j] = (double)power;
     while (!a->interleaved && d / 2 % v) v >>= 1;
     at += d / 2;
     a->first[x + 1] = at;
@@ -371,9 +394,10 @@ int build_norm(const ecnf_qk_norm* o, bool grad, Norm* a, int* ve, bool pointers
   for (int k = 0; k < 2; ++k) {
     NormSide& s = a->s[k];
     if (!s.tokens) continue;
-    // tokens of a tile: about 4 rows a lane group, unless that leaves fewer than 1024 tiles; their angles fit the LDS
-    const int64_t want = (4 * 256 / a->lp + s.H - 1) / s.H, few = (s.tokens + 1023) / 1024;
-    int64_t tt = want < few ? want : few;
+    // tokens of a tile: about 4 rows a lane group, unless that leaves fewer than 1024 tiles (then fewer, but a row for
+    // every lane group); their angles fit the LDS
+    const int64_t want = (4 * 256 / a->lp + s.H - 1) / s.H, few = (s.tokens + 1023) / 1024, one = (256 / a->lp + s.H - 1) / s.H;
+    int64_t tt = want < few ? want : few < one ? one : few;
     if (tt > kCsEntries / a->half) tt = kCsEntries / a->half;
     while (tt > 1 && tt * s.H > (1 << 24)) --tt;
     s.tt = (int)(tt < 1 ? 1 : tt);
@@ -413,7 +437,7 @@ int run_norm(const ecnf_qk_norm* o, void* ws, size_t bytes, void* stream) {
     else if (o->dtype == ECNF_DTYPE_BF16) launch_norm<__bf16, GRAD>(a, ve, (unsigned)grid, s);
     else launch_norm<_Float16, GRAD>(a, ve, (unsigned)grid, s);
   }
-  if (GRAD && dw) qk_norm_dw_kernel<<<dim3((a.D + 15) / 16, 2), 256, 0, s>>>(a);
+  if (GRAD && dw) qk_norm_dw_kernel<<<dim3((a.D + 15) / 16, 2), 1024, 0, s>>>(a);
   const hipError_t e = hipGetLastError();
   return e == hipSuccess ? ECNF_OK : hip_fail(e);
 }
