@@ -37,6 +37,13 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
+// waves a SIMD: at least LOW (what the kernel's registers allow without spills); at head_dim 128 exactly that many, so
+// that the scheduler spends the registers on reads ahead (long bf16 forward 1031 -> 1023 us), and elsewhere as many as
+// fit (at head_dim 64 three instead of four make the 333-key forward 40 us of 35)
+#define ECNF_WAVES(LOW) __attribute__((amdgpu_waves_per_eu((LOW), DP < 128 ? 8 : (LOW))))
+constexpr int waves(int dp, int bytes, int at32, int at64) {
+  return bytes == 4 ? (dp == 32 ? 3 : dp == 64 ? 2 : 1) : dp == 32 ? at32 : dp == 64 ? at64 : 2;
+}
 #define ECNF_LDS(T) __attribute__((address_space(3))) T
 
 template <int V>
@@ -359,31 +366,26 @@ __device__ __forceinline__ void store4(char* p, f32x4 v) {
 // one row block join their statistics and outputs through LDS at the end.  grid = contexts * key heads * tiles * splits;
 // with splits > 1 a workgroup takes its share of the key tiles and leaves a normalised fp32 partial and its lse.
 // ---------------------------------------------------------------------------------------------------------------
-template <class T, int DP, int WR, int WK, int KT>
+template <class T, int DP, int WR, int WK, int KT, int BUFS>
 struct FwdShape {
   static constexpr int kKeys = WK * KT;
   static constexpr int kTileBytes = kKeys * DP * (int)sizeof(T);
   // two buffers of K, V and the keys' bias; where the waves split the keys, the join reuses them: O of every wave, m, l
   static constexpr int kBuf = 2 * kTileBytes;
-  static constexpr int kBufs = 2 * (kBuf + kKeys * 4) <= 160 * 1024 ? 2 : 1;
+  static constexpr int kBufs = BUFS * (kBuf + kKeys * 4) <= 160 * 1024 ? BUFS : 1;
   static constexpr int kBias = kBufs * kBuf;   // the biases lie behind the tiles (which start on multiples of 512 bytes)
   static constexpr int kLoop = kBias + kBufs * kKeys * 4;
   static constexpr int kJoin = WK > 1 ? 4 * 32 * DP * 4 + 4 * 64 * 4 : 0;
   static constexpr int kLds = kLoop > kJoin ? kLoop : kJoin;
 };
 
-// waves a SIMD that the registers are to leave room for
-template <class T, int DP, int RB>
-constexpr int fwd_waves() { return sizeof(T) == 4 ? 1 : RB * DP > 128 ? 1 : 2; }
-
-template <class T, int DP, int WR, int WK, int KT, int RB>
-__global__ __launch_bounds__(256, (fwd_waves<T, DP, RB>())) void att_fwd(Att a) {
-  typedef FwdShape<T, DP, WR, WK, KT> Sh;
-  constexpr int kKeys = Sh::kKeys, NS = DP / 16, ND = DP / 32, NB = KT / 32, kRows = 32 * WR * RB;
+template <class T, int DP, int WR, int WK, int KT, int BUFS>
+__global__ __launch_bounds__(256) ECNF_WAVES(waves(DP, sizeof(T), 4, 4)) void att_fwd(Att a) {
+  typedef FwdShape<T, DP, WR, WK, KT, BUFS> Sh;
+  constexpr int kKeys = Sh::kKeys, NS = DP / 16, ND = DP / 32, NB = KT / 32, kRows = 32 * WR;
   constexpr int64_t e = (int64_t)sizeof(T);
-  static_assert(WK == 1 || RB == 1, "the join has one row block a wave");
   extern __shared__ __attribute__((aligned(1024))) char lds[];
-  const int tid = threadIdx.x, l = tid & 63, w = wave_id(), h = l >> 5, wr = w % WR, wk = w / WR;
+  const int tid = threadIdx.x, l = tid & 63, w = wave_id(), h = l >> 5, wr = WR == 1 ? 0 : w % WR, wk = WK == 1 ? 0 : w / WR;
   int id = xcd_order(blockIdx.x, gridDim.x);
   const int tile = id % a.tiles;
   id /= a.tiles;
@@ -391,26 +393,21 @@ __global__ __launch_bounds__(256, (fwd_waves<T, DP, RB>())) void att_fwd(Att a) 
   id /= a.splits;
   const int hk = id % a.Hk, c = id / a.Hk;
 
-  const int r0 = tile * kRows + wr * 32 * RB + (l & 31);   // row of block x: r0 + 32 x
+  const int r = tile * kRows + wr * 32 + (l & 31);
   // a negative scale turns the queries (exact); 0 becomes a scale under which every score rounds to 0
   const float sc = fmaxf(fabsf(a.scale) * kLog2e, 1e-30f);
-  typename Ops<T>::Frag qf[RB][NS];
-  bool live[RB];
+  int b = 0, i = 0, g = 0;
+  bool live = r < a.R;
+  if (live) {
+    row_of(a, c, r, b, i, g);
+    live = row_live(a, b, i);
+  }
+  const char* qrow = live ? a.q + ((int64_t)b * a.qs[0] + (int64_t)i * a.qs[1] + (int64_t)(hk * a.G + g) * a.qs[2]) * e : nullptr;
+  typename Ops<T>::Frag qf[NS];
 #pragma unroll
-  for (int x = 0; x < RB; ++x) {
-    const int r = r0 + 32 * x;
-    int b = 0, i = 0, g = 0;
-    live[x] = r < a.R;
-    if (live[x]) {
-      row_of(a, c, r, b, i, g);
-      live[x] = row_live(a, b, i);
-    }
-    const char* qrow = live[x] ? a.q + ((int64_t)b * a.qs[0] + (int64_t)i * a.qs[1] + (int64_t)(hk * a.G + g) * a.qs[2]) * e : nullptr;
-#pragma unroll
-    for (int s = 0; s < NS; ++s) {
-      qf[x][s] = frag_global<T>(qrow, s, h, a.D);
-      if (a.scale < 0.f) qf[x][s] = -qf[x][s];
-    }
+  for (int s = 0; s < NS; ++s) {
+    qf[s] = frag_global<T>(qrow, s, h, a.D);
+    if (a.scale < 0.f) qf[s] = -qf[s];
   }
 
   const int n = key_count(a, c);
@@ -432,15 +429,11 @@ __global__ __launch_bounds__(256, (fwd_waves<T, DP, RB>())) void att_fwd(Att a) 
     if (!whole(t) && tid < kKeys) biases[buf * kKeys + tid] = allowed(t * kKeys + tid) ? 0.f : -kInf;
   };
 
-  f32x16 o[RB][ND];
-  float m[RB], sum[RB];
+  f32x16 o[ND];
+  float m = -kInf, sum = 0.f;
 #pragma unroll
-  for (int x = 0; x < RB; ++x) {
-    m[x] = -kInf, sum[x] = 0.f;
-#pragma unroll
-    for (int d = 0; d < ND; ++d) o[x][d] = f32x16{};
-  }
-  const bool idle = tile * kRows + wr * 32 * RB >= a.R;
+  for (int d = 0; d < ND; ++d) o[d] = f32x16{};
+  const bool idle = tile * kRows + wr * 32 >= a.R;
   const float slack = 8.f / sc;   // P may reach 2^8 before the running maximum moves (a rescale of O less often)
   if (t0 < t1) fetch(t0, 0);
   auto step = [&](int t, auto which) {
@@ -451,71 +444,55 @@ __global__ __launch_bounds__(256, (fwd_waves<T, DP, RB>())) void att_fwd(Att a) 
     const uint32_t kat = cur * Sh::kBuf, vat = kat + Sh::kTileBytes;
     const float* bias = biases + cur * kKeys;
     if (!idle && (WK == 1 || t * kKeys + wk * KT < n)) {   // the wave has rows, and keys of this tile
-    f32x16 sx[RB][NB];
+      f32x16 sx[NB];
 #pragma unroll
-    for (int kb = 0; kb < NB; ++kb) {
+      for (int kb = 0; kb < NB; ++kb) {
+        sx[kb] = f32x16{};
 #pragma unroll
-      for (int x = 0; x < RB; ++x) sx[x][kb] = f32x16{};
-#pragma unroll
-      for (int s = 0; s < NS; ++s) {
-        const auto kf = rd.frag(kat, wk * KT + kb * 32, s);
-#pragma unroll
-        for (int x = 0; x < RB; ++x) sx[x][kb] = Ops<T>::mma(kf, qf[x][s], sx[x][kb]);
+        for (int s = 0; s < NS; ++s) sx[kb] = Ops<T>::mma(rd.frag(kat, wk * KT + kb * 32, s), qf[s], sx[kb]);
       }
-    }
-    if (!whole(t)) {
+      if (!whole(t)) {
 #pragma unroll
-      for (int kb = 0; kb < NB; ++kb)
+        for (int kb = 0; kb < NB; ++kb)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const f32x4 bs = *reinterpret_cast<const f32x4*>(bias + wk * KT + kb * 32 + 8 * j + 4 * h);
+          for (int j = 0; j < 4; ++j) {
+            const f32x4 bs = *reinterpret_cast<const f32x4*>(bias + wk * KT + kb * 32 + 8 * j + 4 * h);
 #pragma unroll
-          for (int y = 0; y < 4; ++y)
-#pragma unroll
-            for (int x = 0; x < RB; ++x) sx[x][kb][4 * j + y] += bs[y];
-        }
-    }
-#pragma unroll
-    for (int x = 0; x < RB; ++x) {
+            for (int y = 0; y < 4; ++y) sx[kb][4 * j + y] += bs[y];
+          }
+      }
       float mx = -kInf;
 #pragma unroll
       for (int kb = 0; kb < NB; ++kb)
 #pragma unroll
-        for (int y = 0; y < 16; ++y) mx = fmaxf(mx, sx[x][kb][y]);
+        for (int y = 0; y < 16; ++y) mx = fmaxf(mx, sx[kb][y]);
       mx = max_halves(mx);
-      if (__any(mx > m[x] + slack)) {
-        const float mn = fmaxf(m[x], mx);
-        const float al = __builtin_amdgcn_exp2f((m[x] - (mn == -kInf ? 0.f : mn)) * sc);
-        sum[x] *= al;
+      if (__any(mx > m + slack)) {
+        const float mn = fmaxf(m, mx);
+        const float al = __builtin_amdgcn_exp2f((m - (mn == -kInf ? 0.f : mn)) * sc);
+        sum *= al;
 #pragma unroll
         for (int d = 0; d < ND; ++d)
 #pragma unroll
-          for (int y = 0; y < 16; ++y) o[x][d][y] *= al;
-        m[x] = mn;
+          for (int y = 0; y < 16; ++y) o[d][y] *= al;
+        m = mn;
       }
-      const float ref = m[x] == -kInf ? 0.f : -m[x] * sc;   // nothing allowed yet: exp2(-inf) = 0
+      const float ref = m == -kInf ? 0.f : -m * sc;   // nothing allowed yet: exp2(-inf) = 0
 #pragma unroll
       for (int kb = 0; kb < NB; ++kb)
 #pragma unroll
         for (int y = 0; y < 16; ++y) {
-          sx[x][kb][y] = __builtin_amdgcn_exp2f(fmaf(sx[x][kb][y], sc, ref));
-          sum[x] += sx[x][kb][y];
+          sx[kb][y] = __builtin_amdgcn_exp2f(fmaf(sx[kb][y], sc, ref));
+          sum += sx[kb][y];
         }
-    }
 #pragma unroll
-    for (int kb = 0; kb < NB; ++kb)
+      for (int kb = 0; kb < NB; ++kb)
 #pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        typename Ops<T>::Frag p[RB];
+        for (int s = 0; s < 2; ++s) {
+          const auto p = to_frag<T>(sx[kb], s);
 #pragma unroll
-        for (int x = 0; x < RB; ++x) p[x] = to_frag<T>(sx[x][kb], s);
-#pragma unroll
-        for (int d = 0; d < ND; ++d) {
-          const auto vf = rd.frag_t(vat, wk * KT + kb * 32 + 16 * s, d);
-#pragma unroll
-          for (int x = 0; x < RB; ++x) o[x][d] = Ops<T>::mma(vf, p[x], o[x][d]);
+          for (int d = 0; d < ND; ++d) o[d] = Ops<T>::mma(rd.frag_t(vat, wk * KT + kb * 32 + 16 * s, d), p, o[d]);
         }
-      }
     }
     if (Sh::kBufs == 1 && t + 1 < t1) {
       __syncthreads();
@@ -541,37 +518,34 @@ __global__ __launch_bounds__(256, (fwd_waves<T, DP, RB>())) void att_fwd(Att a) 
     else if (a.lse) a.lse[((int64_t)bb * a.Hq + hk * a.G + gg) * a.Lq + ii] = lse * kLn2;
   };
   if constexpr (WK == 1) {
-#pragma unroll
-    for (int x = 0; x < RB; ++x) {
-      const int r = r0 + 32 * x;
-      const float tot = sum_halves(sum[x]);
-      const float inv = tot > 0.f ? 1.f / tot : (tot == 0.f ? 0.f : tot);   // NaN stays
-      if (r >= a.R) continue;
-      int b, i, g;
+    const float tot = sum_halves(sum);
+    const float inv = tot > 0.f ? 1.f / tot : (tot == 0.f ? 0.f : tot);   // NaN stays
+    if (r < a.R) {
       row_of(a, c, r, b, i, g);
 #pragma unroll
       for (int d = 0; d < ND; ++d)
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const int dd = 32 * d + 8 * j + 4 * h;
-          const f32x16& y = o[x][d];
-          if (dd < a.D) put(r, live[x], b, i, g, dd, f32x4{y[4 * j] * inv, y[4 * j + 1] * inv, y[4 * j + 2] * inv, y[4 * j + 3] * inv});
+          if (dd < a.D)
+            put(r, live, b, i, g, dd,
+                f32x4{o[d][4 * j] * inv, o[d][4 * j + 1] * inv, o[d][4 * j + 2] * inv, o[d][4 * j + 3] * inv});
         }
-      if (h == 0) put_lse(r, live[x], b, i, g, m[x], tot);
+      if (h == 0) put_lse(r, live, b, i, g, m, tot);
     }
   } else {
     float* jo = reinterpret_cast<float*>(lds);                 // [wave][row][DP], 16-byte chunks swizzled by row
     float* jm = jo + 4 * 32 * DP;                              // [wave][row]
     float* jl = jm + 4 * 32;
-    const float tot = sum_halves(sum[0]);
+    const float tot = sum_halves(sum);
     __syncthreads();
 #pragma unroll
     for (int d = 0; d < ND; ++d)
 #pragma unroll
       for (int j = 0; j < 4; ++j)
         *reinterpret_cast<f32x4*>(reinterpret_cast<char*>(jo + w * 32 * DP) + Tile<float, DP>::at(l & 31, 8 * d + 2 * j + h)) =
-            f32x4{o[0][d][4 * j], o[0][d][4 * j + 1], o[0][d][4 * j + 2], o[0][d][4 * j + 3]};
-    if (h == 0) jm[w * 32 + (l & 31)] = m[0], jl[w * 32 + (l & 31)] = tot;
+            f32x4{o[d][4 * j], o[d][4 * j + 1], o[d][4 * j + 2], o[d][4 * j + 3]};
+    if (h == 0) jm[w * 32 + (l & 31)] = m, jl[w * 32 + (l & 31)] = tot;
     __syncthreads();
     for (int x = tid; x < WR * 32 * (DP / 4); x += 256) {
       const int ch = x % (DP / 4), row = x / (DP / 4), rw = row >> 5, rl = row & 31;
@@ -642,12 +616,12 @@ __global__ __launch_bounds__(256) void att_fwd_join(Att a) {
 // registers.  Also writes every row's delta and lse (log2 units; +inf for a row without keys, whose P is then 0) for
 // the kernel below.
 // ---------------------------------------------------------------------------------------------------------------
-template <class T, int DP, int WR, int WK, int KT>
-__global__ __launch_bounds__(256, sizeof(T) == 4 ? 1 : 2) void att_dq(Att a) {
-  typedef FwdShape<T, DP, WR, WK, KT> Sh;
+template <class T, int DP, int WR, int WK, int KT, int BUFS>
+__global__ __launch_bounds__(256) ECNF_WAVES(waves(DP, sizeof(T), 4, 3)) void att_dq(Att a) {
+  typedef FwdShape<T, DP, WR, WK, KT, BUFS> Sh;
   constexpr int kKeys = Sh::kKeys, NS = DP / 16, ND = DP / 32, NB = KT / 32;
   extern __shared__ __attribute__((aligned(1024))) char lds[];
-  const int tid = threadIdx.x, l = tid & 63, w = tid >> 6, h = l >> 5, wr = w % WR, wk = w / WR;
+  const int tid = threadIdx.x, l = tid & 63, w = wave_id(), h = l >> 5, wr = WR == 1 ? 0 : w % WR, wk = WK == 1 ? 0 : w / WR;
   int id = xcd_order(blockIdx.x, gridDim.x);
   const int tile = id % a.tiles;
   id /= a.tiles;
@@ -832,12 +806,12 @@ struct DkvShape {
 };
 
 template <class T, int DP, int WY, int WX>
-__global__ __launch_bounds__(256, sizeof(T) == 4 ? 1 : 2) void att_dkv(Att a) {
+__global__ __launch_bounds__(256) ECNF_WAVES(waves(DP, sizeof(T), 3, 2)) void att_dkv(Att a) {
   typedef DkvShape<T, DP, WY, WX> Sh;
   constexpr int kRows = Sh::kRows, NS = DP / 16, ND = DP / 32;
   constexpr int64_t e = (int64_t)sizeof(T);
   extern __shared__ __attribute__((aligned(1024))) char lds[];
-  const int tid = threadIdx.x, l = tid & 63, w = wave_id(), h = l >> 5, wy = w % WY, wx = w / WY;
+  const int tid = threadIdx.x, l = tid & 63, w = wave_id(), h = l >> 5, wy = WY == 1 ? 0 : w % WY, wx = WX == 1 ? 0 : w / WY;
   int id = xcd_order(blockIdx.x, gridDim.x);
   const int tile = id % a.tiles;
   id /= a.tiles;
@@ -1036,6 +1010,7 @@ constexpr int64_t kPartMax = 64ll << 20;
 
 struct Plan {
   int narrow;    // 1: the waves split the inner dimension (few rows / few keys), 0: the outer one
+  int single;    // narrow: one tile buffer (few tiles: more workgroups fit a CU), 0: two (the next tile loads meanwhile)
   int tiles, splits;
   int64_t grid, part, part_lse;   // workgroups; workspace floats
 };
@@ -1056,6 +1031,7 @@ inline Plan make_plan(int64_t pairs, int outer, int inner, int narrow_step, int 
   const int64_t one = pairs * outer * per_row;
   if (one > 0 && s * one > kPartMax) s = kPartMax / one;
   p.splits = (int)(s < 1 ? 1 : s);
+  p.single = inner_tiles <= 2 * p.splits;
   p.grid = base * p.splits;
   p.part = p.splits > 1 ? (int64_t)p.splits * one : 0;
   p.part_lse = p.splits > 1 && lse ? (int64_t)p.splits * pairs * outer : 0;
