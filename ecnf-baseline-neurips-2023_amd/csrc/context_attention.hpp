@@ -40,10 +40,13 @@ typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 // waves a SIMD: at least LOW (what the kernel's registers allow without spills); at head_dim 128 exactly that many, so
 // that the scheduler spends the registers on reads ahead (long bf16 forward 1031 -> 1023 us), and elsewhere as many as
 // fit (at head_dim 64 three instead of four make the 333-key forward 40 us of 35)
-#define ECNF_WAVES(LOW) __attribute__((amdgpu_waves_per_eu((LOW), DP < 128 ? 8 : (LOW))))
-constexpr int waves(int dp, int bytes, int at32, int at64) {
-  return bytes == 4 ? (dp == 32 ? 3 : dp == 64 ? 2 : 1) : dp == 32 ? at32 : dp == 64 ? at64 : 2;
+#define ECNF_WAVES(LOW) __attribute__((amdgpu_waves_per_eu((LOW), HD <= 64 ? 8 : (LOW))))
+constexpr int waves(int hd, int bytes, int at32, int at64) {
+  return bytes == 4 ? (hd <= 32 ? 3 : hd <= 64 ? 2 : 1) : hd <= 32 ? at32 : hd <= 64 ? at64 : 2;
 }
+// The kernels are compiled for head_dim up to HD = 16, 32, 64, 96 and 128 (steps of 16 in the scores, blocks of 32 in
+// the outputs); LDS rows are the next power of two.
+constexpr int tile_width(int hd) { return hd <= 32 ? 32 : hd <= 64 ? 64 : 128; }
 #define ECNF_LDS(T) __attribute__((address_space(3))) T
 
 template <int V>
@@ -379,10 +382,11 @@ struct FwdShape {
   static constexpr int kLds = kLoop > kJoin ? kLoop : kJoin;
 };
 
-template <class T, int DP, int WR, int WK, int KT, int BUFS>
-__global__ __launch_bounds__(256) ECNF_WAVES(waves(DP, sizeof(T), 4, 4)) void att_fwd(Att a) {
+template <class T, int HD, int WR, int WK, int KT, int BUFS>
+__global__ __launch_bounds__(256) ECNF_WAVES(waves(HD, sizeof(T), 4, 4)) void att_fwd(Att a) {
+  constexpr int DP = tile_width(HD);
   typedef FwdShape<T, DP, WR, WK, KT, BUFS> Sh;
-  constexpr int kKeys = Sh::kKeys, NS = DP / 16, ND = DP / 32, NB = KT / 32, kRows = 32 * WR;
+  constexpr int kKeys = Sh::kKeys, NS = HD / 16, ND = (HD + 31) / 32, NB = KT / 32, kRows = 32 * WR;
   constexpr int64_t e = (int64_t)sizeof(T);
   extern __shared__ __attribute__((aligned(1024))) char lds[];
   const int tid = threadIdx.x, l = tid & 63, w = wave_id(), h = l >> 5, wr = WR == 1 ? 0 : w % WR, wk = WK == 1 ? 0 : w / WR;
@@ -616,10 +620,11 @@ __global__ __launch_bounds__(256) void att_fwd_join(Att a) {
 // registers.  Also writes every row's delta and lse (log2 units; +inf for a row without keys, whose P is then 0) for
 // the kernel below.
 // ---------------------------------------------------------------------------------------------------------------
-template <class T, int DP, int WR, int WK, int KT, int BUFS>
-__global__ __launch_bounds__(256) ECNF_WAVES(waves(DP, sizeof(T), 4, 3)) void att_dq(Att a) {
+template <class T, int HD, int WR, int WK, int KT, int BUFS>
+__global__ __launch_bounds__(256) ECNF_WAVES(waves(HD, sizeof(T), 4, 3)) void att_dq(Att a) {
+  constexpr int DP = tile_width(HD);
   typedef FwdShape<T, DP, WR, WK, KT, BUFS> Sh;
-  constexpr int kKeys = Sh::kKeys, NS = DP / 16, ND = DP / 32, NB = KT / 32;
+  constexpr int kKeys = Sh::kKeys, NS = HD / 16, ND = (HD + 31) / 32, NB = KT / 32;
   extern __shared__ __attribute__((aligned(1024))) char lds[];
   const int tid = threadIdx.x, l = tid & 63, w = wave_id(), h = l >> 5, wr = WR == 1 ? 0 : w % WR, wk = WK == 1 ? 0 : w / WR;
   int id = xcd_order(blockIdx.x, gridDim.x);
@@ -805,10 +810,11 @@ struct DkvShape {
   static constexpr int kLds = kLoop > kJoin ? kLoop : kJoin;
 };
 
-template <class T, int DP, int WY, int WX>
-__global__ __launch_bounds__(256) ECNF_WAVES(waves(DP, sizeof(T), 3, 2)) void att_dkv(Att a) {
+template <class T, int HD, int WY, int WX>
+__global__ __launch_bounds__(256) ECNF_WAVES(waves(HD, sizeof(T), 3, 2)) void att_dkv(Att a) {
+  constexpr int DP = tile_width(HD);
   typedef DkvShape<T, DP, WY, WX> Sh;
-  constexpr int kRows = Sh::kRows, NS = DP / 16, ND = DP / 32;
+  constexpr int kRows = Sh::kRows, NS = HD / 16, ND = (HD + 31) / 32;
   constexpr int64_t e = (int64_t)sizeof(T);
   extern __shared__ __attribute__((aligned(1024))) char lds[];
   const int tid = threadIdx.x, l = tid & 63, w = wave_id(), h = l >> 5, wy = WY == 1 ? 0 : w % WY, wx = WX == 1 ? 0 : w / WY;
