@@ -67,58 +67,34 @@ __device__ __forceinline__ float2 cos_sin(double t) {
   return make_float2((k == 1 || k == 2) ? -a : a, (k & 2) ? -b : b);
 }
 
-template <class T, int VE>
-struct Vec {
-  static __device__ __forceinline__ void load(const char* p, float* v) {
-    typedef T V __attribute__((ext_vector_type(VE)));
-    if constexpr (VE == 1) {
-      v[0] = (float)*reinterpret_cast<const T*>(p);
-    } else {
-      const V x = *reinterpret_cast<const V*>(p);
-#pragma unroll
-      for (int i = 0; i < VE; ++i) v[i] = (float)x[i];
-    }
+// a lane's VE pairs of a row as loaded: [lo .., hi ..], or 2 VE neighbours (interleaved)
+template <class T, int VE, bool inter>
+struct Pairs {
+  typedef T V __attribute__((ext_vector_type(VE)));
+  V u, v;
+  __device__ __forceinline__ void load(const char* row, int lo, int hi) {
+    u = *reinterpret_cast<const V*>(row + lo * (int)sizeof(T));
+    v = *reinterpret_cast<const V*>(row + (inter ? lo + VE : hi) * (int)sizeof(T));
   }
-  static __device__ __forceinline__ void store(char* p, const float* v) {
-    typedef T V __attribute__((ext_vector_type(VE)));
-    if constexpr (VE == 1) {
-      *reinterpret_cast<T*>(p) = (T)v[0];
-    } else {
-      V x;
-#pragma unroll
-      for (int i = 0; i < VE; ++i) x[i] = (T)v[i];
-      *reinterpret_cast<V*>(p) = x;
-    }
+  __device__ __forceinline__ void store(char* row, int lo, int hi) const {
+    *reinterpret_cast<V*>(row + lo * (int)sizeof(T)) = u;
+    *reinterpret_cast<V*>(row + (inter ? lo + VE : hi) * (int)sizeof(T)) = v;
   }
+  __device__ __forceinline__ void get(float* a, float* b) const {
+#pragma unroll
+    for (int i = 0; i < VE; ++i) a[i] = (float)at(inter ? 2 * i : i), b[i] = (float)at(inter ? 2 * i + 1 : VE + i);
+  }
+  __device__ __forceinline__ void set(const float* a, const float* b) {
+    T w[2 * VE];
+#pragma unroll
+    for (int i = 0; i < VE; ++i)
+      if (inter) w[2 * i] = (T)a[i], w[2 * i + 1] = (T)b[i];
+      else w[i] = (T)a[i], w[VE + i] = (T)b[i];
+#pragma unroll
+    for (int i = 0; i < VE; ++i) u[i] = w[i], v[i] = w[VE + i];
+  }
+  __device__ __forceinline__ T at(int i) const { return i < VE ? u[i] : v[i - VE]; }
 };
-
-// a lane's VE pairs: first elements in a, second ones in b
-template <class T, int VE>
-__device__ __forceinline__ void load_pairs(const char* row, bool inter, int lo, int hi, float* a, float* b) {
-  if (inter) {
-    float v[2 * VE];
-    Vec<T, VE>::load(row + lo * (int)sizeof(T), v);
-    Vec<T, VE>::load(row + (lo + VE) * (int)sizeof(T), v + VE);
-#pragma unroll
-    for (int i = 0; i < VE; ++i) a[i] = v[2 * i], b[i] = v[2 * i + 1];
-  } else {
-    Vec<T, VE>::load(row + lo * (int)sizeof(T), a);
-    Vec<T, VE>::load(row + hi * (int)sizeof(T), b);
-  }
-}
-template <class T, int VE>
-__device__ __forceinline__ void store_pairs(char* row, bool inter, int lo, int hi, const float* a, const float* b) {
-  if (inter) {
-    float v[2 * VE];
-#pragma unroll
-    for (int i = 0; i < VE; ++i) v[2 * i] = a[i], v[2 * i + 1] = b[i];
-    Vec<T, VE>::store(row + lo * (int)sizeof(T), v);
-    Vec<T, VE>::store(row + (lo + VE) * (int)sizeof(T), v + VE);
-  } else {
-    Vec<T, VE>::store(row + lo * (int)sizeof(T), a);
-    Vec<T, VE>::store(row + hi * (int)sizeof(T), b);
-  }
-}
 
 __device__ __forceinline__ int axis_of(const Norm& a, int pair) {   // n_axes: not rotated
   int x = 0;
@@ -126,9 +102,9 @@ __device__ __forceinline__ int axis_of(const Norm& a, int pair) {   // n_axes: n
   return x;
 }
 
-template <class T, int VE, bool GRAD>
+template <class T, int VE, bool inter, bool GRAD>
 __global__ __launch_bounds__(256) void qk_norm_kernel(Norm a) {
-  constexpr int U = GRAD ? 1 : 2;
+  constexpr int U = GRAD ? 1 : 2;   // (two in the backward pass: 104 us of 96 at 453 MB, its registers halve the waves)
   __shared__ float2 cs[kCsEntries];
   __shared__ float red[GRAD ? 256 * 2 * VE : 1];
   const int tid = threadIdx.x;
@@ -138,7 +114,6 @@ __global__ __launch_bounds__(256) void qk_norm_kernel(Norm a) {
   const int ln = tid & (a.lp - 1), slot = tid / a.lp, slots = 256 / a.lp;
   const int p0 = ln * VE;
   const bool on = p0 < a.half;
-  const bool inter = a.interleaved;
   int lo = 2 * p0, hi = lo;
   if (!inter && on) {
     const int x = axis_of(a, p0), f0 = x ? a.first[x] : 0, n = (x < a.n_axes ? a.first[x + 1] : a.half) - f0;
@@ -154,25 +129,11 @@ __global__ __launch_bounds__(256) void qk_norm_kernel(Norm a) {
     ga[i] = gb[i] = 0.f;
   }
   for (int tile = block; tile < s.tiles; tile += s.blocks) {
-    const int tok0 = tile * s.tt, nt = min(s.tt, s.tokens - tok0);
-    if (GRAD) __syncthreads();
-    for (int x = tid; x < nt * a.half; x += 256) {
-      const int tt = x / a.half, p = x - tt * a.half;
-      const int ax = axis_of(a, p);
-      float2 v = make_float2(1.f, 0.f);
-      if (ax < a.n_axes) {
-        const int tok = tok0 + tt, b = (int)s.dL.div(tok), i = tok - b * s.L;
-        const char* pp = s.pos + ((int64_t)b * s.ps[0] + (int64_t)i * s.ps[1] + ax) * (s.pos_type == ECNF_POS_I64 ? 8 : 4);
-        v = cos_sin(position(s, pp) * a.turns[p]);
-      }
-      cs[x] = v;
-    }
-    __syncthreads();
-    const int rows = nt * s.H;
-    for (int rs = slot; rs < rows; rs += U * slots) {
-      // U rows at once: their loads are in flight together
-      float xa[U][VE], xb[U][VE], da[U][VE], db[U][VE];
-      int tt[U], head[U];
+    const int tok0 = tile * s.tt, nt = min(s.tt, s.tokens - tok0), rows = nt * s.H;
+    // U rows at once: their loads are in flight together, the first ones while the angles are made
+    Pairs<T, VE, inter> px[U], pd[GRAD ? U : 1];
+    int tt[U], head[U];
+    auto fetch = [&](int rs) __attribute__((always_inline)) {
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         const int rr = min(rs + u * slots, rows - 1);   // behind the last row: read again, not written
@@ -180,29 +141,48 @@ __global__ __launch_bounds__(256) void qk_norm_kernel(Norm a) {
         head[u] = rr - tt[u] * s.H;
         const int tok = tok0 + tt[u], b = (int)s.dL.div(tok), i = tok - b * s.L;
         if (on) {
-          load_pairs<T, VE>(s.x + ((int64_t)b * s.xs[0] + (int64_t)i * s.xs[1] + (int64_t)head[u] * s.xs[2]) * (int64_t)sizeof(T), inter, lo, hi, xa[u], xb[u]);
-          if (GRAD)
-            load_pairs<T, VE>(s.dy + ((int64_t)b * s.gs[0] + (int64_t)i * s.gs[1] + (int64_t)head[u] * s.gs[2]) * (int64_t)sizeof(T), inter, lo, hi, da[u], db[u]);
-        } else {
-#pragma unroll
-          for (int q = 0; q < VE; ++q) xa[u][q] = xb[u][q] = da[u][q] = db[u][q] = 0.f;
+          px[u].load(s.x + ((int64_t)b * s.xs[0] + (int64_t)i * s.xs[1] + (int64_t)head[u] * s.xs[2]) * (int64_t)sizeof(T), lo, hi);
+          if constexpr (GRAD)
+            pd[u].load(s.dy + ((int64_t)b * s.gs[0] + (int64_t)i * s.gs[1] + (int64_t)head[u] * s.gs[2]) * (int64_t)sizeof(T), lo, hi);
         }
       }
+    };
+    fetch(slot);
+    if (GRAD) __syncthreads();
+    for (int x = tid; x < nt * a.half; x += 256) {
+      const int t = x / a.half, p = x - t * a.half;
+      const int ax = axis_of(a, p);
+      float2 v = make_float2(1.f, 0.f);
+      if (ax < a.n_axes) {
+        const int tok = tok0 + t, b = (int)s.dL.div(tok), i = tok - b * s.L;
+        const char* pp = s.pos + ((int64_t)b * s.ps[0] + (int64_t)i * s.ps[1] + ax) * (s.pos_type == ECNF_POS_I64 ? 8 : 4);
+        v = cos_sin(position(s, pp) * a.turns[p]);
+      }
+      cs[x] = v;
+    }
+    __syncthreads();
+    for (int rs = slot; rs < rows; rs += U * slots) {
+      if (rs != slot) fetch(rs);
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         float2 t[VE];
 #pragma unroll
         for (int q = 0; q < VE; ++q) t[q] = on ? cs[tt[u] * a.half + p0 + q] : make_float2(1.f, 0.f);
-        float ya[VE], yb[VE], ss = 0.f, dot = 0.f;
+        float xa[VE], xb[VE], ya[VE], yb[VE], ss = 0.f, dot = 0.f;
+        px[u].get(xa, xb);
+        if constexpr (GRAD) {
+          float da[VE], db[VE];
+          pd[u].get(da, db);
 #pragma unroll
-        for (int q = 0; q < VE; ++q) {
-          ss = fmaf(xa[u][q], xa[u][q], fmaf(xb[u][q], xb[u][q], ss));
-          if (GRAD) {
-            ya[q] = fmaf(da[u][q], t[q].x, db[u][q] * t[q].y);
-            yb[q] = fmaf(db[u][q], t[q].x, -(da[u][q] * t[q].y));
-            dot = fmaf(ya[q] * wa[q], xa[u][q], fmaf(yb[q] * wb[q], xb[u][q], dot));
+          for (int q = 0; q < VE; ++q) {
+            ya[q] = fmaf(da[q], t[q].x, db[q] * t[q].y);
+            yb[q] = fmaf(db[q], t[q].x, -(da[q] * t[q].y));
+            dot = fmaf(ya[q] * wa[q], xa[q], fmaf(yb[q] * wb[q], xb[q], dot));
           }
         }
+#pragma unroll
+        for (int q = 0; q < VE; ++q) ss = fmaf(xa[q], xa[q], fmaf(xb[q], xb[q], ss));
+        if (!on) ss = dot = 0.f;   // lanes beside the row hold nothing
         for (int m = a.lp >> 1; m; m >>= 1) {
           ss += __shfl_xor(ss, m);
           if (GRAD) dot += __shfl_xor(dot, m);
@@ -214,20 +194,22 @@ __global__ __launch_bounds__(256) void qk_norm_kernel(Norm a) {
           const float m = r * r * (dot / (float)a.D);
 #pragma unroll
           for (int q = 0; q < VE; ++q) {
-            ga[q] = fmaf(ya[q], xa[u][q] * r, ga[q]);
-            gb[q] = fmaf(yb[q], xb[u][q] * r, gb[q]);
-            ya[q] = r * (ya[q] * wa[q] - xa[u][q] * m);
-            yb[q] = r * (yb[q] * wb[q] - xb[u][q] * m);
+            ga[q] = fmaf(ya[q], xa[q] * r, ga[q]);
+            gb[q] = fmaf(yb[q], xb[q] * r, gb[q]);
+            ya[q] = r * (ya[q] * wa[q] - xa[q] * m);
+            yb[q] = r * (yb[q] * wb[q] - xb[q] * m);
           }
         } else {
 #pragma unroll
           for (int q = 0; q < VE; ++q) {
-            const float x = xa[u][q] * r * wa[q], y = xb[u][q] * r * wb[q];
+            const float x = xa[q] * r * wa[q], y = xb[q] * r * wb[q];
             ya[q] = fmaf(x, t[q].x, -(y * t[q].y));
             yb[q] = fmaf(x, t[q].y, y * t[q].x);
           }
         }
-        store_pairs<T, VE>(o, inter, lo, hi, ya, yb);
+        Pairs<T, VE, inter> out;
+        out.set(ya, yb);
+        out.store(o, lo, hi);
       }
     }
   }
@@ -407,13 +389,18 @@ int build_norm(const ecnf_qk_norm* o, bool grad, Norm* a, int* ve, bool pointers
   return ECNF_OK;
 }
 
+template <class T, bool GRAD, int VE>
+void launch_norm(const Norm& a, unsigned grid, hipStream_t s) {
+  if (a.interleaved) qk_norm_kernel<T, VE, true, GRAD><<<grid, 256, 0, s>>>(a);
+  else qk_norm_kernel<T, VE, false, GRAD><<<grid, 256, 0, s>>>(a);
+}
 template <class T, bool GRAD>
 void launch_norm(const Norm& a, int ve, unsigned grid, hipStream_t s) {
   if (ve == 8) {
-    if constexpr (sizeof(T) == 2) qk_norm_kernel<T, 8, GRAD><<<grid, 256, 0, s>>>(a);
-  } else if (ve == 4) qk_norm_kernel<T, 4, GRAD><<<grid, 256, 0, s>>>(a);
-  else if (ve == 2) qk_norm_kernel<T, 2, GRAD><<<grid, 256, 0, s>>>(a);
-  else qk_norm_kernel<T, 1, GRAD><<<grid, 256, 0, s>>>(a);
+    if constexpr (sizeof(T) == 2) launch_norm<T, GRAD, 8>(a, grid, s);
+  } else if (ve == 4) launch_norm<T, GRAD, 4>(a, grid, s);
+  else if (ve == 2) launch_norm<T, GRAD, 2>(a, grid, s);
+  else launch_norm<T, GRAD, 1>(a, grid, s);
 }
 
 template <bool GRAD>

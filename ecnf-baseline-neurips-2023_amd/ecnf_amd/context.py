@@ -33,7 +33,8 @@ _POSITIONS = {torch.int32: _lib.POS_I32, torch.int64: _lib.POS_I64, torch.float3
 # filling a ctypes structure field by field (tests/test_context.py holds them to the compiled library's layout)
 _QK_NORM = struct.Struct("@" + 2 * "6P8q4i" + "9ifd")
 _ATTENTION = struct.Struct("@12P12q9if")
-_NO_SIDE = (0,) * 18
+_CONTIGUOUS = torch.contiguous_format
+_NO_SIDE, _NO_STRIDES, _NO_AXES = (0,) * 18, (0,) * 3, (0,) * 4
 
 
 def _tensor(x, name: str, like: Optional[torch.Tensor] = None) -> torch.Tensor:
@@ -53,8 +54,8 @@ def _tensor(x, name: str, like: Optional[torch.Tensor] = None) -> torch.Tensor:
 
 def _strides(x: torch.Tensor) -> Tuple[int, int, int]:
     """Strides of the first three dimensions; 0 where there is one element (torch's may be anything there)."""
-    n, s = x.shape, x.stride()
-    return (s[0] if n[0] > 1 else 0, s[1] if n[1] > 1 else 0, s[2] if n[2] > 1 else 0)
+    (a, b, c, d), (sa, sb, sc, _) = x.shape, x.stride()
+    return (sa if a > 1 else 0, sb if b > 1 else 0, sc if c > 1 else 0)
 
 
 def _aligned(x: torch.Tensor) -> torch.Tensor:
@@ -71,7 +72,7 @@ def _stream(device: torch.device) -> int:
 
 
 def _new(x: torch.Tensor) -> torch.Tensor:
-    return torch.empty_like(x, memory_format=torch.contiguous_format)
+    return torch.empty_like(x, memory_format=_CONTIGUOUS)
 
 
 def _same_shape(x: torch.Tensor, like: torch.Tensor, name: str) -> None:
@@ -80,65 +81,67 @@ def _same_shape(x: torch.Tensor, like: torch.Tensor, name: str) -> None:
 
 
 # ------------------------------------------------------------------------------------------------------ norm + rotation
-def _weight(w, x: torch.Tensor, name: str) -> Optional[torch.Tensor]:
-    if w is None:
-        return None
+def _weight(w, x: torch.Tensor, name: str) -> torch.Tensor:
     if not (torch.is_tensor(w) and w.device == x.device and w.dim() == 1 and w.shape[0] == x.shape[3]
             and w.dtype in _DTYPES):
         raise ValueError(f"{name} must be a floating [head_dim = {x.shape[3]}] tensor on {x.device}")
-    return w.float().contiguous()
+    return w if w.dtype == torch.float32 and w.is_contiguous() else w.float().contiguous()
 
 
 def _positions(p, x: torch.Tensor, n_axes: int, name: str) -> Tuple[torch.Tensor, int, int]:
     """(positions, batch stride, token stride)"""
     if not (torch.is_tensor(p) and p.device == x.device and p.dtype in _POSITIONS):
         raise ValueError(f"{name} must be an int32, int64 or float32 tensor on {x.device}")
-    B, L = x.shape[0], x.shape[1]
-    if tuple(p.shape) not in ((L, n_axes), (B, L, n_axes)):
-        raise ValueError(f"{name} must be [{L}, {n_axes}] or [{B}, {L}, {n_axes}], got {tuple(p.shape)}")
-    if p.stride(-1) != 1 and n_axes > 1:
+    n, shape = p.dim(), p.shape
+    if not (2 <= n <= 3 and shape[-1] == n_axes and shape[-2] == x.shape[1] and (n == 2 or shape[0] == x.shape[0])):
+        raise ValueError(f"{name} must be [{x.shape[1]}, {n_axes}] or [{x.shape[0]}, {x.shape[1]}, {n_axes}], got "
+                         f"{tuple(shape)}")
+    st = p.stride()
+    if st[-1] != 1 and n_axes > 1:
         p = p.contiguous()
-    return p, (p.stride(0) if p.dim() == 3 else 0), p.stride(-2)
+        st = p.stride()
+    return p, (st[0] if n == 3 else 0), st[-2]
 
 
-def _norm_call(sides, axes, theta, eps, interleaved, grad: bool):
-    """sides: (x, weight, positions, output gradient or None, name) of q and k; returns (outputs, weight gradients)."""
+def _norm_call(q, k, axes, theta, eps, interleaved, grad: bool):
+    """q, k: (x, weight, positions, output gradient or None, name), k None for none; returns (outputs, weight gradients)."""
     axes = tuple(int(a) for a in axes)
-    if not 1 <= len(axes) <= 4:
+    n_axes = len(axes)
+    if not 1 <= n_axes <= 4:
         raise ValueError("axes must name one to four axes")
-    first = sides[0][0]
-    packed, outs, dws, keep = [], [], [], []
-    for x, w, pos, g, name in sides:
-        if x is None:
+    packed, outs, dws, keep = (), [], [], []
+    for side in (q, k):
+        if side is None:
             packed += _NO_SIDE
             outs.append(None)
             dws.append(None)
             continue
-        w32 = _weight(w, x, f"{name}_weight")
-        p, pb, pl = _positions(pos, x, len(axes), f"{name}_positions")
+        x, w, pos, g, name = side
+        w32 = None if w is None else _weight(w, x, name + "_weight")
+        p, pb, pl = _positions(pos, x, n_axes, name + "_positions")
         out = _new(x)
         dw = torch.empty(x.shape[3], dtype=torch.float32, device=x.device) if grad and w is not None else None
-        gs = (0, 0, 0) if g is None else _strides(g)
-        packed += (x.data_ptr(), 0 if g is None else g.data_ptr(), out.data_ptr(), 0 if w32 is None else w32.data_ptr(),
-                   0 if dw is None else dw.data_ptr(), p.data_ptr(), *_strides(x), *gs, pb, pl,
-                   x.shape[0], x.shape[1], x.shape[2], _POSITIONS[p.dtype])
+        packed += (x.data_ptr(), 0 if g is None else g.data_ptr(), out.data_ptr(), 0 if w is None else w32.data_ptr(),
+                   0 if dw is None else dw.data_ptr(), p.data_ptr(), *_strides(x), *(_NO_STRIDES if g is None else _strides(g)),
+                   pb, pl, *x.shape[:3], _POSITIONS[p.dtype])
         outs.append(out)
         dws.append(dw)
-        keep.append((w32, p))
-    args = _QK_NORM.pack(*packed, _DTYPES[first.dtype], first.shape[3], len(axes), *axes, *(0,) * (4 - len(axes)),
-                         bool(interleaved), first.device.index, eps, theta)
+        keep.append((w32, p))   # alive until the launch
+    x = q[0]
+    device = x.device
+    args = _QK_NORM.pack(*packed, _DTYPES[x.dtype], x.shape[3], n_axes, *(axes + _NO_AXES)[:4], bool(interleaved),
+                         device.index, eps, theta)
     lib = _lib.load()
-    stream = _stream(first.device)
     if not grad:
-        _lib.check(lib.ecnf_qk_norm_rotary(args, stream))
+        _lib.check(lib.ecnf_qk_norm_rotary(args, _stream(device)))
         return outs, dws
     n = ctypes.c_size_t()
     _lib.check(lib.ecnf_qk_norm_workspace_size(args, ctypes.byref(n)))
-    ws = torch.empty(n.value, dtype=torch.uint8, device=first.device)
-    _lib.check(lib.ecnf_qk_norm_rotary_grad(args, ws.data_ptr(), n.value, stream))
-    for k, (x, w, _, _, _) in enumerate(sides):
-        if dws[k] is not None and w.dtype != torch.float32:
-            dws[k] = dws[k].to(w.dtype)
+    ws = torch.empty(n.value, dtype=torch.uint8, device=device)
+    _lib.check(lib.ecnf_qk_norm_rotary_grad(args, ws.data_ptr(), n.value, _stream(device)))
+    for i, side in enumerate((q, k)):
+        if dws[i] is not None and side[1].dtype != torch.float32:
+            dws[i] = dws[i].to(side[1].dtype)
     return outs, dws
 
 
@@ -155,8 +158,9 @@ def qk_norm_rotary(q, k=None, *, q_positions, k_positions=None, axes: Sequence[i
         k = _tensor(k, "k", q)
         if k.shape[3] != q.shape[3]:
             raise ValueError(f"k must have q's head_dim {q.shape[3]}, got {k.shape[3]}")
-    outs, _ = _norm_call(((q, q_weight, q_positions, None, "q"), (k, k_weight, k_positions, None, "k")), axes,
-                         float(theta), float(eps), interleaved, False)
+    outs, _ = _norm_call((q, q_weight, q_positions, None, "q"),
+                         None if k is None else (k, k_weight, k_positions, None, "k"), axes, float(theta), float(eps),
+                         interleaved, False)
     return outs[0], outs[1]
 
 
@@ -174,8 +178,9 @@ def qk_norm_rotary_grad(q_grad, k_grad, q, k=None, *, q_positions, k_positions=N
             raise ValueError(f"k must have q's head_dim {q.shape[3]}, got {k.shape[3]}")
         k_grad = _tensor(k_grad, "k_grad", q)
         _same_shape(k_grad, k, "k_grad")
-    outs, dws = _norm_call(((q, q_weight, q_positions, q_grad, "q"), (k, k_weight, k_positions, k_grad, "k")), axes,
-                           float(theta), float(eps), interleaved, True)
+    outs, dws = _norm_call((q, q_weight, q_positions, q_grad, "q"),
+                           None if k is None else (k, k_weight, k_positions, k_grad, "k"), axes, float(theta),
+                           float(eps), interleaved, True)
     return outs[0], outs[1], dws[0], dws[1]
 
 
@@ -221,7 +226,7 @@ def _attention_args(q, k, v, out, dout, lse, dq, dk, dv, ql, cl, m, scale) -> by
         return 0 if t is None else t.data_ptr()
     return _ATTENTION.pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), ptr(dout), ptr(lse), ptr(dq), ptr(dk),
                            ptr(dv), ptr(ql), ptr(cl), ptr(m), *_strides(q), *_strides(k), *_strides(v),
-                           *((0, 0, 0) if dout is None else _strides(dout)), _DTYPES[q.dtype], B, C, Lq, Lk, Hq, Hk, D,
+                           *(_NO_STRIDES if dout is None else _strides(dout)), _DTYPES[q.dtype], B, C, Lq, Lk, Hq, Hk, D,
                            q.device.index, scale)
 
 
