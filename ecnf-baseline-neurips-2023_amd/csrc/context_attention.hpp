@@ -129,10 +129,6 @@ __device__ __forceinline__ typename Ops<T>::Frag to_frag(const f32x16& x, int s)
   return f;
 }
 
-__device__ __forceinline__ float other_half(float x) {   // the value of lane ^ 32
-  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-  return __uint_as_float((threadIdx.x & 32) ? r[0] : r[1]);
-}
 __device__ __forceinline__ float max_halves(float x) {
   const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
   return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
@@ -141,6 +137,44 @@ __device__ __forceinline__ float sum_halves(float x) {
   const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
   return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
+
+// The backward pass in fp16.  P is about 1 / keys and dS smaller still, at or below fp16's subnormals in long contexts
+// (1 / 16384 = 2^-14), so both are rounded as multiples of a power of two, which the accumulators carry: kPScale for P
+// (at most 1, so at most 2^14), and for dS one a column (row of dQ, key of dK), moved as the largest |dS| so far needs it.
+// What is rounded away is then 2^-12 of the value, or 2^-39 of the column's largest.
+constexpr float kPScale = 16384.f;
+template <class T>
+struct Range {   // types with fp32's exponents need nothing
+  __device__ __forceinline__ void fit(f32x16&, f32x16*, int) {}
+  __device__ __forceinline__ float back() const { return 1.f; }
+  static constexpr float kP = 1.f;
+};
+template <>
+struct Range<_Float16> {
+  static constexpr float kP = kPScale;
+  float scale = 0x1p120f;
+  // scales x (one column a lane, its other rows in the other half), and the accumulators where the scale moves
+  __device__ __forceinline__ void fit(f32x16& x, f32x16* acc, int n) {
+    float m = 0.f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) m = fmaxf(m, fabsf(x[i]));
+    m = max_halves(m);
+    if (__any(m * scale > 32768.f)) {
+      // the largest lands in [2^14, 2^15); an infinity or NaN stays one
+      const int e = (int)(__float_as_uint(m) >> 23);
+      const float want = __uint_as_float((uint32_t)min(max(268 - e, 1), 254) << 23);
+      const float next = fminf(scale, want), move = next / scale;
+      scale = next;
+#pragma unroll
+      for (int d = 0; d < n; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) acc[d][i] *= move;
+    }
+#pragma unroll
+    for (int i = 0; i < 16; ++i) x[i] *= scale;
+  }
+  __device__ __forceinline__ float back() const { return 1.f / scale; }
+};
 
 // A row-major tile in LDS, rows of DP elements, its 16-byte chunks swizzled inside a row: chunk c of row r sits at
 // c ^ f(r).  f takes 16 rows to 16 different groups of 4 banks (64 banks: fragment reads, 16 lanes of 16 rows, meet no
@@ -690,6 +724,7 @@ __global__ __launch_bounds__(256) ECNF_WAVES(waves(HD, sizeof(T), 4, 3)) void at
   };
 
   const bool idle = tile * 32 * WR + wr * 32 >= a.R;
+  Range<T> range;
   f32x16 acc[ND];
 #pragma unroll
   for (int d = 0; d < ND; ++d) acc[d] = f32x16{};
@@ -726,6 +761,7 @@ __global__ __launch_bounds__(256) ECNF_WAVES(waves(HD, sizeof(T), 4, 3)) void at
         const float p = __builtin_amdgcn_exp2f(fmaf(sx[x], sc, -lse));
         sx[x] = p * (dp[x] - delta);
       }
+      range.fit(sx, acc, ND);
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
         const auto dsf = to_frag<T>(sx, s);
@@ -744,6 +780,11 @@ __global__ __launch_bounds__(256) ECNF_WAVES(waves(HD, sizeof(T), 4, 3)) void at
     if (Sh::kBufs == 2 && t + 1 < t1) step(t + 1, Const<1>{});
   }
 
+  if constexpr (Range<T>::kP != 1.f) {
+    const float back = range.back();
+#pragma unroll
+    for (int d = 0; d < ND; ++d) acc[d] *= back;
+  }
   const int64_t n_rows = (int64_t)a.C * a.Hk * a.R, row0 = ((int64_t)c * a.Hk + hk) * a.R;
   auto put = [&](int rr, bool lv, int bb, int ii, int gg, int d, f32x4 v) {
     if (rr >= a.R) return;
@@ -865,6 +906,7 @@ __global__ __launch_bounds__(256) ECNF_WAVES(waves(HD, sizeof(T), 3, 2)) void at
 
   float* const stats = reinterpret_cast<float*>(lds + Sh::kStat);
   const bool idle = (tile * WY + wy) * 32 >= n;
+  Range<T> range;
   const bool fast = a.flat && !a.qlen && kRows % a.G == 0;
   RowTile<T, DP, kRows> tq, td;
   tq.init(a, a.q, a.qs, c, hk, tid, fast);
@@ -915,10 +957,11 @@ __global__ __launch_bounds__(256) ECNF_WAVES(waves(HD, sizeof(T), 3, 2)) void at
         for (int x = 0; x < 4; ++x) {
           float p = __builtin_amdgcn_exp2f(fmaf(sx[4 * j + x], sc, -ls[x]));
           p = ok ? p : 0.f;
-          sx[4 * j + x] = p;
+          sx[4 * j + x] = p * Range<T>::kP;
           dp[4 * j + x] = p * (dp[4 * j + x] - de[x]);
         }
       }
+      range.fit(dp, dk, ND);
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
         const auto pf = to_frag<T>(sx, s), sf = to_frag<T>(dp, s);
@@ -938,6 +981,11 @@ __global__ __launch_bounds__(256) ECNF_WAVES(waves(HD, sizeof(T), 3, 2)) void at
     }
   }
 
+  if constexpr (Range<T>::kP != 1.f) {
+    const float back = range.back();
+#pragma unroll
+    for (int d = 0; d < ND; ++d) dk[d] *= back, dv[d] *= 1.f / kPScale;
+  }
   const int64_t n_keys = (int64_t)a.C * a.Hk * a.Lk;
   auto put = [&](int which, int kk, int d, f32x4 v) {
     if (kk >= a.Lk || d >= a.D) return;

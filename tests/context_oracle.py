@@ -1,7 +1,8 @@
 """Plain 64-bit forms of the context operators and how far the kernels may be from them.
 
 The bounds are first-order sums of the roundings a kernel makes: u = half a step of the operand type (P, dS, outputs),
-e = 2^-24 (every fp32 operation), d = 2^-25 (fp16 operands: half of the smallest subnormal, absolute).
+e = 2^-24 (every fp32 operation), d = 2^-25 (fp16: half of the smallest subnormal, absolute: the outputs, and the
+forward pass's P, which is at least 1 somewhere in its row; the backward pass scales its P and dS by powers of two).
 """
 import math
 
@@ -76,11 +77,13 @@ def attention(q, k, v, query_lengths=None, context_lengths=None, context_mask=No
     eP = eP + 2 * t_lse
     t_delta = (G.abs() * (tO + D * E * O.abs())).sum(-1, keepdim=True)
     t_dP = (D + 2) * E * (G.abs() @ V.abs().transpose(2, 3))
-    tS = (up + eP + 4 * E) * dS.abs() + P * (t_dP + t_delta) + d * (P > 0)
+    # fp16: what a column's scale cuts off is 2^-39 of its largest dS
+    cut = 2.0 ** -39 if q.dtype == torch.float16 else 0.0
+    tS = (up + eP + 4 * E) * dS.abs() + P * (t_dP + t_delta) + cut * (dS.abs().amax((2, 3), keepdim=True) if Lk else 0.0)
     n = Q.shape[2]
     tQ = abs(scale) * (tS + (Lk + 2) * E * dS.abs()) @ K.abs()
     tK = abs(scale) * (tS + (n + 2) * E * dS.abs()).transpose(2, 3) @ Q.abs()
-    tV = ((up + eP + (n + 2) * E) * P + d * (P > 0)).transpose(2, 3) @ G.abs()
+    tV = ((up + eP + (n + 2) * E) * P + cut * (P > 0)).transpose(2, 3) @ G.abs()
     dQ, dK, dV = scale * dS @ K, scale * dS.transpose(2, 3) @ Q, P.transpose(2, 3) @ G
     res["dq"] = (back(dQ), back(tQ + u * dQ.abs() + d))
     res["dk"] = tuple(x.permute(0, 2, 1, 3) for x in (dK, tK + u * dK.abs() + d))

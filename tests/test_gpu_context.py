@@ -144,11 +144,11 @@ ATT = [  # B, Lq, Hq, C, Lk, Hk, D
 ]
 
 
-def attention_case(C, dtype, shape, lengths, mask, queries, seed=0, scale=None, values=1.0):
+def attention_case(C, dtype, shape, lengths, mask, queries, seed=0, scale=None, grads=1.0):
     B, Lq, Hq, Ck, Lk, Hk, D = shape
     g = gen(seed)
-    q, do = normal(g, B, Lq, Hq, D, dtype=dtype), normal(g, B, Lq, Hq, D, dtype=dtype)
-    k, v = normal(g, Ck, Lk, Hk, D, dtype=dtype), values * normal(g, Ck, Lk, Hk, D, dtype=dtype)
+    q, do = normal(g, B, Lq, Hq, D, dtype=dtype), (grads * normal(g, B, Lq, Hq, D)).to(dtype)
+    k, v = normal(g, Ck, Lk, Hk, D, dtype=dtype), normal(g, Ck, Lk, Hk, D, dtype=dtype)
     kw = dict(scale=scale)
     if lengths:
         n = torch.randint(0, Lk + 1, (Ck,), generator=g, device="cuda", dtype=torch.int32)
@@ -203,6 +203,26 @@ def test_attention_masks(C, dtype, shape, lengths, mask, queries):
     attention_case(C, dtype, shape, lengths, mask, queries, seed=1)
 
 
+@pytest.mark.parametrize("dtype", TYPES, ids=ids)
+@pytest.mark.parametrize("grads", [1e-3, 300.0])
+@pytest.mark.parametrize("shape", [(1, 40, 2, 1, 6000, 2, 64), (1, 4, 2, 1, 6000, 1, 32), (1, 3000, 2, 1, 20, 2, 128)], ids=str)
+def test_attention_small_and_large_gradients(C, dtype, grads, shape):
+    """dS far below and far above 1 (in fp16 below its subnormals): long contexts make P small, the loss scales dO."""
+    attention_case(C, dtype, shape, False, False, False, seed=2, grads=grads)
+
+
+def test_attention_gradients_of_very_different_rows(C):
+    """fp16: rows whose gradients differ by 2^20 share a key's sums, and keys far apart a row's."""
+    g = gen(14)
+    q, k, v = (normal(g, 1, n, 2, 64, dtype=torch.float16) for n in (200, 700, 700))
+    do = (normal(g, 1, 200, 2, 64) * 2.0 ** torch.linspace(-14, 6, 200, device="cuda").round()[None, :, None, None]).half()
+    v = (v.float() * 2.0 ** torch.linspace(5, -5, 700, device="cuda").round()[None, :, None, None]).half()
+    want = O.attention(q, k, v, out_grad=do)
+    out, lse = C.cross_attention(q, k, v, return_lse=True)
+    for name, got in zip(("dq", "dk", "dv"), C.cross_attention_grad(do, q, k, v, out, lse)):
+        O.check(name, got, *want[name])
+
+
 def test_attention_sharp_scores(C):
     """Scores far apart: one key takes everything, in a tile that comes late (the running maximum moves every tile)."""
     q = torch.full((1, 2, 1, 32), 2.0, device="cuda")
@@ -212,6 +232,14 @@ def test_attention_sharp_scores(C):
     want = O.attention(q, k, v, scale=1.0)
     O.check("out", out, *want["out"])
     O.check("lse", lse, *want["lse"])
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.3, 3.0])
+def test_attention_scales(C, scale):
+    """No scale (an average over the allowed keys), a negative one and a large one."""
+    for dtype in TYPES:
+        attention_case(C, dtype, (3, 20, 2, 3, 150, 2, 32), True, True, False, seed=3, scale=scale)
+        attention_case(C, dtype, (1, 70, 2, 1, 150, 2, 32), False, False, False, seed=3, scale=scale)
 
 
 def test_attention_differences(C):
