@@ -247,7 +247,7 @@ __device__ __forceinline__ int xcd_order(int b, int n) {
 }
 
 __device__ __forceinline__ int key_count(const Att& a, int c) {
-  return a.klen ? max(0, min(a.klen[c], a.Lk)) : a.Lk;
+  return a.klen ? __builtin_amdgcn_readfirstlane(max(0, min(a.klen[c], a.Lk))) : a.Lk;
 }
 
 // row r of context c -> its molecule and token (r < R)
@@ -263,12 +263,17 @@ __device__ __forceinline__ bool row_live(const Att& a, int b, int i) { return !a
 // Tiles go from memory to LDS without passing registers (16-byte LDS loads): a wave's 64 chunks land consecutively, so
 // the lane that fills slot c' of row r asks for chunk c' ^ f(r).  Issued through asm (the compiler would otherwise make
 // every later LDS read wait for them); dma_wait before the barrier that publishes them.
+__device__ __forceinline__ u32x4 uniform(u32x4 x) {   // the same in every lane, so that it can sit in scalar registers
+#pragma unroll
+  for (int i = 0; i < 4; ++i) x[i] = __builtin_amdgcn_readfirstlane(x[i]);
+  return x;
+}
 __device__ __forceinline__ void dma_buffer(uint32_t lds, u32x4 rsrc, uint32_t off) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(off), "s"(rsrc)
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(__builtin_amdgcn_readfirstlane(lds)), "v"(off), "s"(rsrc)
                : "memory", "m0");
 }
 __device__ __forceinline__ void dma_global(uint32_t lds, const char* p) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(p) : "memory", "m0");
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(__builtin_amdgcn_readfirstlane(lds)), "v"(p) : "memory", "m0");
 }
 __device__ __forceinline__ void dma_wait() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 __device__ __forceinline__ uint32_t lds_address(const void* p) { return (uint32_t)(uintptr_t)(ECNF_LDS(const void)*)p; }
@@ -303,12 +308,12 @@ struct KeyTile {
   __device__ __forceinline__ void load(uint32_t lds, int k0, int valid, bool masked, Allowed allowed) const {
     const uint64_t p = (uint64_t)(base + (int64_t)k0 * stride);
     const int rows = min(valid, ROWS);
-    const u32x4 rsrc = {(uint32_t)p, (uint32_t)(p >> 32) & 0xffffu, (uint32_t)(rows - 1) * stride + (uint32_t)end, 0x00020000u};
+    const u32x4 rsrc = uniform(u32x4{(uint32_t)p, (uint32_t)(p >> 32) & 0xffffu, (uint32_t)(rows - 1) * stride + (uint32_t)end, 0x00020000u});
     const uint32_t at = lds + wave_id() * 1024;
 #pragma unroll
     for (int n = 0; n < kN; ++n) {
       uint32_t o = off[n % kAlt] + (uint32_t)(n / kAlt * kAlt * kStep) * stride;
-      if (masked) o = allowed(k0 + row + n * kStep) ? o : kBehind;
+      if (masked) o = allowed(row + n * kStep) ? o : kBehind;
       dma_buffer(at + n * 4096, rsrc, o);
     }
   }
@@ -347,7 +352,7 @@ struct RowTile {
     const uint32_t at = lds + wave_id() * 1024;
     if (fast) {
       const uint64_t p = (uint64_t)(base + (int64_t)a.dG.div((uint32_t)r0) * s1);
-      const u32x4 rsrc = {(uint32_t)p, (uint32_t)(p >> 32) & 0xffffu, 0x7ffffff0u, 0x00020000u};
+      const u32x4 rsrc = uniform(u32x4{(uint32_t)p, (uint32_t)(p >> 32) & 0xffffu, 0x7ffffff0u, 0x00020000u});
       const bool tail = r0 + ROWS > a.R;
 #pragma unroll
       for (int n = 0; n < kN; ++n) {
@@ -409,11 +414,81 @@ struct FwdShape {
   static constexpr int kTileBytes = kKeys * DP * (int)sizeof(T);
   // two buffers of K, V and the keys' bias; where the waves split the keys, the join reuses them: O of every wave, m, l
   static constexpr int kBuf = 2 * kTileBytes;
-  static constexpr int kBufs = BUFS * (kBuf + kKeys * 4) <= 160 * 1024 ? BUFS : 1;
+  static constexpr int kBufs = BUFS * kBuf + 3 * kKeys * 4 <= 160 * 1024 ? BUFS : 1;
   static constexpr int kBias = kBufs * kBuf;   // the biases lie behind the tiles (which start on multiples of 512 bytes)
-  static constexpr int kLoop = kBias + kBufs * kKeys * 4;
+  static constexpr int kLoop = kBias + 3 * kKeys * 4;
   static constexpr int kJoin = WK > 1 ? 4 * 32 * DP * 4 + 4 * 64 * 4 : 0;
   static constexpr int kLds = kLoop > kJoin ? kLoop : kJoin;
+};
+
+// The key tiles t0 .. t1 of a workgroup: K and V into the tile buffers, and which keys count.  A tile that is not whole
+// (its end, or any tile under a mask) has a bias of 0 or -inf a key in a ring of three: under a mask the lanes that ask
+// for a masked row behind the range read it while the tile after next's mask bytes are on their way, so no load waits
+// for another (333 masked keys, 44 rows: 25 us unmasked; 36 with the mask read where it is used).
+template <class T, int DP, class Sh>
+struct KeyStream {
+  static constexpr int kKeys = Sh::kKeys;
+  KeyTile<T, DP, kKeys> kt, vt;
+  const uint8_t* mask;
+  float* ring;
+  uint32_t lds0;
+  int n, t0, t1, tid, slot;   // slot: the ring's entry of the current tile
+  float ahead;
+  __device__ __forceinline__ void init(const Att& a, int c, int hk, int split, char* lds, int tid_) {
+    constexpr int64_t e = (int64_t)sizeof(T);
+    tid = tid_;
+    lds0 = lds_address(lds);
+    ring = reinterpret_cast<float*>(lds + Sh::kBias);
+    n = key_count(a, c);
+    const int nt = (n + kKeys - 1) / kKeys, share = (nt + a.splits - 1) / a.splits;
+    t0 = min(split * share, nt);
+    t1 = min(t0 + share, nt);
+    mask = a.mask ? a.mask + (int64_t)c * a.Lk : nullptr;
+    kt.init(a.k + ((int64_t)c * a.ks[0] + (int64_t)hk * a.ks[2]) * e, a.ks[1] * e, a.D, tid);
+    vt.init(a.v + ((int64_t)c * a.vs[0] + (int64_t)hk * a.vs[2]) * e, a.vs[1] * e, a.D, tid);
+  }
+  __device__ __forceinline__ bool whole(int t) const { return !mask && (t + 1) * kKeys <= n; }
+  __device__ __forceinline__ float bias_of(int t) const {
+    const int key = t * kKeys + tid;
+    return key < n && (!mask || mask[key]) ? 0.f : -kInf;
+  }
+  __device__ __forceinline__ const float* bias() const { return ring + slot * kKeys; }
+  // tile t, the ring's entry `at`, into buffer `buf`
+  __device__ __forceinline__ void fetch(int t, int at, int buf) {
+    float* b = ring + at * kKeys;
+    auto allowed = [&](int row) { return b[row] == 0.f; };
+    kt.load(lds0 + buf * Sh::kBuf, t * kKeys, n - t * kKeys, mask != nullptr, allowed);
+    vt.load(lds0 + buf * Sh::kBuf + Sh::kTileBytes, t * kKeys, n - t * kKeys, mask != nullptr, allowed);
+    if (!mask && !whole(t) && tid < kKeys) b[tid] = bias_of(t);
+  }
+  __device__ __forceinline__ void start() {
+    slot = 0;
+    if (t0 >= t1) return;
+    if (mask) {
+      if (tid < kKeys) {
+        ring[tid] = bias_of(t0);
+        if (t0 + 1 < t1) ring[kKeys + tid] = bias_of(t0 + 1);
+      }
+      __syncthreads();
+    }
+    fetch(t0, 0, 0);
+  }
+  // around a tile's products: its tile has landed and every wave is done with the one before; the next loads meanwhile
+  __device__ __forceinline__ void begin(int t, int cur) {
+    dma_wait();
+    __syncthreads();
+    if (mask && t + 2 < t1 && tid < kKeys) ahead = bias_of(t + 2);
+    if (Sh::kBufs == 2 && t + 1 < t1) fetch(t + 1, next(slot), cur ^ 1);
+  }
+  __device__ __forceinline__ void end(int t) {
+    if (mask && t + 2 < t1 && tid < kKeys) ring[next(next(slot)) * kKeys + tid] = ahead;
+    if (Sh::kBufs == 1 && t + 1 < t1) {
+      __syncthreads();
+      fetch(t + 1, next(slot), 0);
+    }
+    slot = next(slot);
+  }
+  static __device__ __forceinline__ int next(int s) { return s == 2 ? 0 : s + 1; }
 };
 
 template <class T, int HD, int WR, int WK, int KT, int BUFS>
@@ -448,24 +523,10 @@ __global__ __launch_bounds__(256) ECNF_WAVES(waves(HD, sizeof(T), 4, 4)) void at
     if (a.scale < 0.f) qf[s] = -qf[s];
   }
 
-  const int n = key_count(a, c);
-  const int nt = (n + kKeys - 1) / kKeys, share = (nt + a.splits - 1) / a.splits;
-  const int t0 = min(split * share, nt), t1 = min(t0 + share, nt);
-  const uint8_t* mask = a.mask ? a.mask + (int64_t)c * a.Lk : nullptr;
-  auto allowed = [&](int key) { return key < n && (!mask || mask[key]); };
-  KeyTile<T, DP, kKeys> kt, vt;
-  kt.init(a.k + ((int64_t)c * a.ks[0] + (int64_t)hk * a.ks[2]) * e, a.ks[1] * e, a.D, tid);
-  vt.init(a.v + ((int64_t)c * a.vs[0] + (int64_t)hk * a.vs[2]) * e, a.vs[1] * e, a.D, tid);
-  auto whole = [&](int t) { return !mask && (t + 1) * kKeys <= n; };
-  const uint32_t lds0 = lds_address(lds);
+  KeyStream<T, DP, Sh> ks;
+  ks.init(a, c, hk, split, lds, tid);
   Reader<T, DP> rd;
-  rd.init(lds0, l);
-  float* const biases = reinterpret_cast<float*>(lds + Sh::kBias);
-  auto fetch = [&](int t, int buf) {
-    kt.load(lds0 + buf * Sh::kBuf, t * kKeys, n - t * kKeys, mask != nullptr, allowed);
-    vt.load(lds0 + buf * Sh::kBuf + Sh::kTileBytes, t * kKeys, n - t * kKeys, mask != nullptr, allowed);
-    if (!whole(t) && tid < kKeys) biases[buf * kKeys + tid] = allowed(t * kKeys + tid) ? 0.f : -kInf;
-  };
+  rd.init(ks.lds0, l);
 
   f32x16 o[ND];
   float m = -kInf, sum = 0.f;
@@ -473,15 +534,13 @@ __global__ __launch_bounds__(256) ECNF_WAVES(waves(HD, sizeof(T), 4, 4)) void at
   for (int d = 0; d < ND; ++d) o[d] = f32x16{};
   const bool idle = tile * kRows + wr * 32 >= a.R;
   const float slack = 8.f / sc;   // P may reach 2^8 before the running maximum moves (a rescale of O less often)
-  if (t0 < t1) fetch(t0, 0);
+  ks.start();
   auto step = [&](int t, auto which) {
     constexpr int cur = decltype(which)::value;
-    dma_wait();
-    __syncthreads();   // tile t has landed, and every wave is done with tile t - 1
-    if (Sh::kBufs == 2 && t + 1 < t1) fetch(t + 1, cur ^ 1);
+    ks.begin(t, cur);
     const uint32_t kat = cur * Sh::kBuf, vat = kat + Sh::kTileBytes;
-    const float* bias = biases + cur * kKeys;
-    if (!idle && (WK == 1 || t * kKeys + wk * KT < n)) {   // the wave has rows, and keys of this tile
+    const float* bias = ks.bias();
+    if (!idle && (WK == 1 || t * kKeys + wk * KT < ks.n)) {   // the wave has rows, and keys of this tile
       f32x16 sx[NB];
 #pragma unroll
       for (int kb = 0; kb < NB; ++kb) {
@@ -489,7 +548,7 @@ __global__ __launch_bounds__(256) ECNF_WAVES(waves(HD, sizeof(T), 4, 4)) void at
 #pragma unroll
         for (int s = 0; s < NS; ++s) sx[kb] = Ops<T>::mma(rd.frag(kat, wk * KT + kb * 32, s), qf[s], sx[kb]);
       }
-      if (!whole(t)) {
+      if (!ks.whole(t)) {
 #pragma unroll
         for (int kb = 0; kb < NB; ++kb)
 #pragma unroll
@@ -532,15 +591,12 @@ __global__ __launch_bounds__(256) ECNF_WAVES(waves(HD, sizeof(T), 4, 4)) void at
           for (int d = 0; d < ND; ++d) o[d] = Ops<T>::mma(rd.frag_t(vat, wk * KT + kb * 32 + 16 * s, d), p, o[d]);
         }
     }
-    if (Sh::kBufs == 1 && t + 1 < t1) {
-      __syncthreads();
-      fetch(t + 1, 0);
-    }
+    ks.end(t);
   };
   // the buffer is a constant of each half: every LDS address is a register of the loop plus a constant offset
-  for (int t = t0; t < t1; t += Sh::kBufs) {
+  for (int t = ks.t0; t < ks.t1; t += Sh::kBufs) {
     step(t, Const<0>{});
-    if (Sh::kBufs == 2 && t + 1 < t1) step(t + 1, Const<1>{});
+    if (Sh::kBufs == 2 && t + 1 < ks.t1) step(t + 1, Const<1>{});
   }
 
   // ---- join the key waves, normalise, store.  lse in log2 units; an empty row has sum 0: output 0, lse -inf
@@ -704,44 +760,28 @@ __global__ __launch_bounds__(256) ECNF_WAVES(waves(HD, sizeof(T), 4, 3)) void at
     a.row_delta[row] = delta;
   }
 
-  const int n = key_count(a, c);
-  const int nt = (n + kKeys - 1) / kKeys, share = (nt + a.splits - 1) / a.splits;
-  const int t0 = min(split * share, nt), t1 = min(t0 + share, nt);
-  const uint8_t* mask = a.mask ? a.mask + (int64_t)c * a.Lk : nullptr;
-  auto allowed = [&](int key) { return key < n && (!mask || mask[key]); };
-  KeyTile<T, DP, kKeys> kt, vt;
-  kt.init(a.k + ((int64_t)c * a.ks[0] + (int64_t)hk * a.ks[2]) * e, a.ks[1] * e, a.D, tid);
-  vt.init(a.v + ((int64_t)c * a.vs[0] + (int64_t)hk * a.vs[2]) * e, a.vs[1] * e, a.D, tid);
-  auto whole = [&](int t) { return !mask && (t + 1) * kKeys <= n; };
-  const uint32_t lds0 = lds_address(lds);
+  KeyStream<T, DP, Sh> ks;
+  ks.init(a, c, hk, split, lds, tid);
   Reader<T, DP> rd;
-  rd.init(lds0, l);
-  float* const biases = reinterpret_cast<float*>(lds + Sh::kBias);
-  auto fetch = [&](int t, int buf) {
-    kt.load(lds0 + buf * Sh::kBuf, t * kKeys, n - t * kKeys, mask != nullptr, allowed);
-    vt.load(lds0 + buf * Sh::kBuf + Sh::kTileBytes, t * kKeys, n - t * kKeys, mask != nullptr, allowed);
-    if (!whole(t) && tid < kKeys) biases[buf * kKeys + tid] = allowed(t * kKeys + tid) ? 0.f : -kInf;
-  };
+  rd.init(ks.lds0, l);
 
   const bool idle = tile * 32 * WR + wr * 32 >= a.R;
   Range<T> range;
   f32x16 acc[ND];
 #pragma unroll
   for (int d = 0; d < ND; ++d) acc[d] = f32x16{};
-  if (t0 < t1) fetch(t0, 0);
+  ks.start();
   auto step = [&](int t, auto which) {
     constexpr int cur = decltype(which)::value;
-    dma_wait();
-    __syncthreads();   // tile t has landed, and every wave is done with tile t - 1
-    if (Sh::kBufs == 2 && t + 1 < t1) fetch(t + 1, cur ^ 1);
+    ks.begin(t, cur);
     const uint32_t kat = cur * Sh::kBuf, vat = kat + Sh::kTileBytes;
-    const float* bias = biases + cur * kKeys;
-    const bool all = whole(t);
+    const float* bias = ks.bias();
+    const bool all = ks.whole(t);
     if (!idle)
 #pragma unroll
     for (int kb = 0; kb < NB; ++kb) {
       const int k0 = wk * KT + kb * 32;
-      if (t * kKeys + k0 >= n) break;
+      if (t * kKeys + k0 >= ks.n) break;
       f32x16 sx = f32x16{}, dp = f32x16{};
 #pragma unroll
       for (int s = 0; s < NS; ++s) {
@@ -769,15 +809,12 @@ __global__ __launch_bounds__(256) ECNF_WAVES(waves(HD, sizeof(T), 4, 3)) void at
         for (int d = 0; d < ND; ++d) acc[d] = Ops<T>::mma(rd.frag_t(kat, k0 + 16 * s, d), dsf, acc[d]);
       }
     }
-    if (Sh::kBufs == 1 && t + 1 < t1) {
-      __syncthreads();
-      fetch(t + 1, 0);
-    }
+    ks.end(t);
   };
   // the buffer is a constant of each half: every LDS address is a register of the loop plus a constant offset
-  for (int t = t0; t < t1; t += Sh::kBufs) {
+  for (int t = ks.t0; t < ks.t1; t += Sh::kBufs) {
     step(t, Const<0>{});
-    if (Sh::kBufs == 2 && t + 1 < t1) step(t + 1, Const<1>{});
+    if (Sh::kBufs == 2 && t + 1 < ks.t1) step(t + 1, Const<1>{});
   }
 
   if constexpr (Range<T>::kP != 1.f) {
@@ -1063,16 +1100,15 @@ __global__ __launch_bounds__(256) void att_grad_join(Att a, int which) {
 constexpr int64_t kPartMax = 64ll << 20;
 
 struct Plan {
-  int narrow;    // 1: the waves split the inner dimension (few rows / few keys), 0: the outer one
-  int single;    // narrow: one tile buffer (few tiles: more workgroups fit a CU), 0: two (the next tile loads meanwhile)
+  int narrow;        // 1: the waves split the loop (few rows / few keys), 0: the rows (forward, dQ) or keys (dK dV)
+  int single;        // one tile buffer (few tiles: more workgroups fit a CU), else two (the next tile loads meanwhile)
   int tiles, splits;
   int64_t grid, part, part_lse;   // workgroups; workspace floats
 };
 
 inline int ceil_div(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
 
-// outer: rows (forward, dQ) or keys (dK dV) of a (context, key head), `inner` the loop's length in elements of
-// `step(narrow)`; per_row: partial floats of one outer element and split.
+// outer: rows (forward, dQ) or keys (dK dV) of a (context, key head); inner: the loop's length, and its tiles'; per_row: partial floats of one outer element and split.
 inline Plan make_plan(int64_t pairs, int outer, int inner, int narrow_step, int wide_step, int64_t per_row, bool lse) {
   Plan p;
   p.narrow = outer <= 32;
