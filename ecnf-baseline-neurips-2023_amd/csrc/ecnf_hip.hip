@@ -1632,7 +1632,14 @@ int integrate_impl(ecnf_handle* h, const ecnf_solve_opts* o, const float* y0, co
     std::lock_guard<std::mutex> tl(h->team_mu);
     if (!h->team_ev) HIP_TRY(hipEventCreateWithFlags(&h->team_ev, hipEventDisableTiming));
     if (h->team_used && h->team_stream != stream) HIP_TRY(hipStreamWaitEvent(stream, h->team_ev, 0));
-    HIP_TRY(dispatch_integrate(h, NT, sp, G, cols, y0, feat, eps, y1, dlogp, nfe, status, batch, stream, nodes));
+    hipError_t e = dispatch_integrate(h, NT, sp, G, cols, y0, feat, eps, y1, dlogp, nfe, status, batch, stream, nodes);
+    if (e == hipErrorIllegalState && h->team_mode.load() == 0) {
+      // no cooperative launch here (another process holds the device's cooperative queue): in auto mode the batch
+      // path, whose results are the same bits
+      (void)hipGetLastError();
+      e = dispatch_integrate(h, NT, sp, 1, 0, y0, feat, eps, y1, dlogp, nfe, status, batch, stream, nodes);
+    }
+    HIP_TRY(e);
     HIP_TRY(hipEventRecord(h->team_ev, stream));
     h->team_used = true;
     h->team_stream = stream;
