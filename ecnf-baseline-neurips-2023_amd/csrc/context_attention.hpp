@@ -416,7 +416,8 @@ struct FwdShape {
   static constexpr int kBuf = 2 * kTileBytes;
   static constexpr int kBufs = BUFS * kBuf + 3 * kKeys * 4 <= 160 * 1024 ? BUFS : 1;
   static constexpr int kBias = kBufs * kBuf;   // the biases lie behind the tiles (which start on multiples of 512 bytes)
-  static constexpr int kLoop = kBias + 3 * kKeys * 4;
+  static constexpr int kDelta = kBias + 3 * kKeys * 4;   // dQ: a sum a row and wave
+  static constexpr int kLoop = kDelta + 4 * 32 * 4;
   static constexpr int kJoin = WK > 1 ? 4 * 32 * DP * 4 + 4 * 64 * 4 : 0;
   static constexpr int kLds = kLoop > kJoin ? kLoop : kJoin;
 };
@@ -754,12 +755,6 @@ __global__ __launch_bounds__(256) ECNF_WAVES(waves(HD, sizeof(T), 4, 3)) void at
     lse = a.lse[((int64_t)b * a.Hq + hq) * a.Lq + i] * kLog2e;
     if (lse == -kInf) lse = kInf;
   }
-  if (split == 0 && wk == 0 && h == 0 && r < a.R) {
-    const int64_t row = ((int64_t)c * a.Hk + hk) * a.R + r;
-    a.row_lse[row] = lse;
-    a.row_delta[row] = delta;
-  }
-
   KeyStream<T, DP, Sh> ks;
   ks.init(a, c, hk, split, lds, tid);
   Reader<T, DP> rd;
@@ -770,37 +765,75 @@ __global__ __launch_bounds__(256) ECNF_WAVES(waves(HD, sizeof(T), 4, 3)) void at
   f32x16 acc[ND];
 #pragma unroll
   for (int d = 0; d < ND; ++d) acc[d] = f32x16{};
+  // P and dP of the 32 keys from k0 of the tile at kat, vat
+  auto products = [&](int t, uint32_t kat, uint32_t vat, int k0, f32x16& p, f32x16& dp) __attribute__((always_inline)) {
+    p = f32x16{}, dp = f32x16{};
+#pragma unroll
+    for (int s = 0; s < NS; ++s) {
+      p = Ops<T>::mma(rd.frag(kat, k0, s), qf[s], p);
+      dp = Ops<T>::mma(rd.frag(vat, k0, s), df[s], dp);
+    }
+    if (!ks.whole(t)) {
+      const float* bias = ks.bias();
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const f32x4 bs = *reinterpret_cast<const f32x4*>(bias + k0 + 8 * j + 4 * h);
+#pragma unroll
+        for (int x = 0; x < 4; ++x) p[4 * j + x] = bs[x] < 0.f ? bs[x] * sg : p[4 * j + x];
+      }
+    }
+#pragma unroll
+    for (int x = 0; x < 16; ++x) p[x] = __builtin_amdgcn_exp2f(fmaf(p[x], sc, -lse));
+  };
   ks.start();
+  // A context of one tile: delta = sum_j P dP over its keys instead of sum_d dO O.  With few keys dP - delta cancels,
+  // and O was rounded (bf16: dQ and dK of 2-key rows 2.6e-3 off, so 1.7e-3, which is their own rounding); with many, O is
+  // an average and its rounding is small beside dP.  The scores are made twice: nothing for 16-bit types (fp32's O is
+  // exact enough; there it would cost 74 -> 79 us of the 22 x 129 training pass).
+  if (sizeof(T) == 2 && ks.t0 < ks.t1 && ks.n <= kKeys) {
+    dma_wait();
+    __syncthreads();
+    float sum = 0.f;
+    if (!idle)
+#pragma unroll
+      for (int kb = 0; kb < NB; ++kb) {
+        const int k0 = wk * KT + kb * 32;
+        if (k0 >= ks.n) break;
+        f32x16 p, dp;
+        products(0, 0, Sh::kTileBytes, k0, p, dp);
+#pragma unroll
+        for (int x = 0; x < 16; ++x) sum = fmaf(p[x], dp[x], sum);
+      }
+    sum = sum_halves(sum);
+    if constexpr (WK == 1) {
+      delta = sum;
+    } else {
+      float* part = reinterpret_cast<float*>(lds + Sh::kDelta);
+      if (h == 0) part[w * 32 + (l & 31)] = sum;
+      __syncthreads();
+      delta = 0.f;
+#pragma unroll
+      for (int k = 0; k < WK; ++k) delta += part[(k * WR + wr) * 32 + (l & 31)];
+    }
+  }
+  if (split == 0 && wk == 0 && h == 0 && r < a.R) {
+    const int64_t row = ((int64_t)c * a.Hk + hk) * a.R + r;
+    a.row_lse[row] = lse;
+    a.row_delta[row] = delta;
+  }
   auto step = [&](int t, auto which) {
     constexpr int cur = decltype(which)::value;
     ks.begin(t, cur);
     const uint32_t kat = cur * Sh::kBuf, vat = kat + Sh::kTileBytes;
-    const float* bias = ks.bias();
-    const bool all = ks.whole(t);
     if (!idle)
 #pragma unroll
     for (int kb = 0; kb < NB; ++kb) {
       const int k0 = wk * KT + kb * 32;
       if (t * kKeys + k0 >= ks.n) break;
-      f32x16 sx = f32x16{}, dp = f32x16{};
+      f32x16 sx, dp;
+      products(t, kat, vat, k0, sx, dp);
 #pragma unroll
-      for (int s = 0; s < NS; ++s) {
-        sx = Ops<T>::mma(rd.frag(kat, k0, s), qf[s], sx);
-        dp = Ops<T>::mma(rd.frag(vat, k0, s), df[s], dp);
-      }
-      if (!all) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const f32x4 bs = *reinterpret_cast<const f32x4*>(bias + k0 + 8 * j + 4 * h);
-#pragma unroll
-          for (int x = 0; x < 4; ++x) sx[4 * j + x] = bs[x] < 0.f ? bs[x] * sg : sx[4 * j + x];
-        }
-      }
-#pragma unroll
-      for (int x = 0; x < 16; ++x) {
-        const float p = __builtin_amdgcn_exp2f(fmaf(sx[x], sc, -lse));
-        sx[x] = p * (dp[x] - delta);
-      }
+      for (int x = 0; x < 16; ++x) sx[x] *= dp[x] - delta;
       range.fit(sx, acc, ND);
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
