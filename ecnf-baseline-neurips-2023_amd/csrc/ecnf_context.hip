@@ -403,6 +403,13 @@ void launch_norm(const Norm& a, int ve, unsigned grid, hipStream_t s) {
   else launch_norm<T, GRAD, 1>(a, grid, s);
 }
 
+// bytes of the backward pass's partials.  The blocks also depend on the operands' alignment: the most there can be
+size_t norm_bytes(const Norm& a) {
+  size_t blocks = 0;
+  for (const NormSide& s : a.s) blocks += s.tokens < kMaxGradBlocks ? s.tokens : kMaxGradBlocks;
+  return blocks * a.D * 4;
+}
+
 template <bool GRAD>
 int run_norm(const ecnf_qk_norm* o, void* ws, size_t bytes, void* stream) {
   Norm a;
@@ -411,7 +418,7 @@ int run_norm(const ecnf_qk_norm* o, void* ws, size_t bytes, void* stream) {
   const int64_t grid = (int64_t)a.s[0].blocks + a.s[1].blocks;
   const bool dw = a.s[0].dw || a.s[1].dw;
   if (GRAD && dw) {
-    if (bytes < (size_t)grid * a.D * 4 || (grid && !ws)) return fail(ECNF_E_INVALID, "workspace below ecnf_qk_norm_workspace_size");
+    if (bytes < norm_bytes(a) || (grid && !ws)) return fail(ECNF_E_INVALID, "workspace below ecnf_qk_norm_workspace_size");
     a.part = (float*)ws;
   }
   if (!grid && !(GRAD && dw)) return ECNF_OK;
@@ -459,6 +466,9 @@ int build_att(const ecnf_attention* o, int what, Att* a, bool pointers) {
   a->dG = fast_div((uint32_t)G);
   a->dL = fast_div((uint32_t)(o->n_queries ? o->n_queries : 1));
   const int e = elem_size(o->dtype);
+  for (const int64_t* st : {o->q_stride, o->k_stride, o->v_stride, what ? o->out_grad_stride : o->q_stride})
+    for (int d = 0; d < 3; ++d)
+      if (st[d] < 0) return fail(ECNF_E_INVALID, "negative stride");
   // tiles of keys are addressed with 32-bit offsets from their first row, tiles of query rows (at most 256) too where
   // the tokens of a context are evenly spaced
   auto span = [&](const int64_t* st, int d) { return st[d] * e * 256 < (1ll << 31); };
@@ -534,10 +544,7 @@ int ecnf_qk_norm_workspace_size(const ecnf_qk_norm* o, size_t* bytes) {
   Norm a;
   int ve;
   if (int rc = build_norm(o, true, &a, &ve, false)) return rc;
-  // the blocks also depend on the operands' alignment: the most there can be
-  size_t blocks = 0;
-  for (const NormSide& s : a.s) blocks += s.tokens < kMaxGradBlocks ? s.tokens : kMaxGradBlocks;
-  *bytes = blocks * a.D * 4;
+  *bytes = norm_bytes(a);
   return ECNF_OK;
 }
 

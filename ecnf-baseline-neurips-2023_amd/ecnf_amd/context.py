@@ -185,13 +185,13 @@ def qk_norm_rotary_grad(q_grad, k_grad, q, k=None, *, q_positions, k_positions=N
 
 
 # ------------------------------------------------------------------------------------------------------ cross attention
-def _lengths(x, n: int, like: torch.Tensor, name: str) -> Optional[torch.Tensor]:
+def _lengths(x, n: int, most: int, like: torch.Tensor, name: str) -> Optional[torch.Tensor]:
     if x is None:
         return None
     if not (torch.is_tensor(x) and x.device == like.device and x.dtype in (torch.int32, torch.int64)
             and tuple(x.shape) == (n,)):
         raise ValueError(f"{name} must be an int32 or int64 [{n}] tensor on {like.device}")
-    return x.to(torch.int32).contiguous()
+    return x.contiguous() if x.dtype == torch.int32 else x.clamp(0, most).to(torch.int32).contiguous()
 
 
 def _attention_operands(q, k, v, query_lengths, context_lengths, context_mask, scale):
@@ -207,8 +207,8 @@ def _attention_operands(q, k, v, query_lengths, context_lengths, context_mask, s
     if Hk < 1 or Hq < 1 or Hq % Hk:
         raise ValueError(f"q's heads ({Hq}) must be a multiple of k's ({Hk})")
     q, k, v = _aligned(q), _aligned(k), _aligned(v)
-    ql = _lengths(query_lengths, B, q, "query_lengths")
-    cl = _lengths(context_lengths, C, q, "context_lengths")
+    ql = _lengths(query_lengths, B, q.shape[1], q, "query_lengths")
+    cl = _lengths(context_lengths, C, Lk, q, "context_lengths")
     m = context_mask
     if m is not None:
         if not (torch.is_tensor(m) and m.device == q.device and m.dtype in (torch.bool, torch.uint8)

@@ -41,6 +41,8 @@ def _attention(**over):
     (dict(head_dim=136), _lib.ECNF_E_UNSUPPORTED), (dict(scale=float("nan")), _lib.ECNF_E_INVALID),
     (dict(scale=float("inf")), _lib.ECNF_E_INVALID),
     (dict(context_batch=1, batch=2 ** 30, n_queries=4), _lib.ECNF_E_UNSUPPORTED),
+    (dict(q_stride=(1024, -64, 64)), _lib.ECNF_E_INVALID), (dict(k_stride=(-1024, 64, 64)), _lib.ECNF_E_INVALID),
+    (dict(v_stride=(1024, 2 ** 23, 64)), _lib.ECNF_E_UNSUPPORTED),
 ])
 def test_attention_refusals_of_both_calls(over, code):
     lib, n = _lib.load(), ctypes.c_size_t()

@@ -223,6 +223,38 @@ def test_attention_gradients_of_very_different_rows(C):
         O.check(name, got, *want[name])
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=ids)
+@pytest.mark.parametrize("rows", [20, 200])
+def test_attention_few_keys(C, dtype, rows):
+    """Two or three keys: dP - delta cancels, but dQ and dK stay as exact as their own rounding and that of dS."""
+    g = gen(15)
+    q, do = normal(g, 64, rows, 2, 64, dtype=dtype), normal(g, 64, rows, 2, 64, dtype=dtype)
+    k, v = normal(g, 64, 3, 2, 64, dtype=dtype), normal(g, 64, 3, 2, 64, dtype=dtype)
+    n = torch.arange(64, device="cuda", dtype=torch.int32) % 2 + 2
+    want = O.attention(q, k, v, context_lengths=n, out_grad=do)
+    out, lse = C.cross_attention(q, k, v, return_lse=True, context_lengths=n)
+    u = O.half_step(dtype)
+    for name, got in zip(("dq", "dk", "dv"), C.cross_attention_grad(do, q, k, v, out, lse, context_lengths=n)):
+        O.check(name, got, *want[name])
+        # two roundings of at most u (uniform in a binade: their rms is at most u / sqrt(3) each), none amplified
+        off = float((got.double() - want[name][0]).norm() / want[name][0].norm())
+        assert off <= 1.5 * math.sqrt(2.0 / 3.0) * u, (name, off)
+
+
+def test_attention_one_key(C):
+    """One key takes all: out is v up to the rounding of exp2(s - m) = 1 (s sc - m sc, one of them rounded) and its division,
+    dV the sum of dO, and dS is 0 up to the roundings of equal products."""
+    g = gen(16)
+    for dtype in TYPES:
+        q, do = normal(g, 2, 40, 2, 32, dtype=dtype), normal(g, 2, 40, 2, 32, dtype=dtype)
+        k, v = normal(g, 2, 1, 2, 32, dtype=dtype), normal(g, 2, 1, 2, 32, dtype=dtype)
+        want = O.attention(q, k, v, out_grad=do)
+        out, lse = C.cross_attention(q, k, v, return_lse=True)
+        grads = C.cross_attention_grad(do, q, k, v, out, lse)
+        for name, got in zip(("out", "dq", "dk", "dv"), (out, *grads)):
+            O.check(name, got, *want[name])
+
+
 def test_attention_sharp_scores(C):
     """Scores far apart: one key takes everything, in a tile that comes late (the running maximum moves every tile)."""
     q = torch.full((1, 2, 1, 32), 2.0, device="cuda")
@@ -341,10 +373,12 @@ def test_captured_and_replayed(C):
 
 def test_lengths_outside_the_range_are_clamped(C):
     q, k = normal(gen(10), 2, 3, 1, 16), normal(gen(11), 2, 40, 1, 16)
-    n = torch.tensor([-5, 10 ** 9], device="cuda")
-    out = C.cross_attention(q, k, k, context_lengths=n)
-    assert float(out[0].abs().max()) == 0.0
-    assert torch.equal(out[1], C.cross_attention(q, k, k)[1])
+    full = C.cross_attention(q, k, k)[1]
+    for n in ([-5, 10 ** 9], [-2 ** 40, 2 ** 40]):
+        n = torch.tensor(n, device="cuda")
+        for x in (n, n.clamp(-2 ** 31, 2 ** 31 - 1).int()):
+            out = C.cross_attention(q, k, k, context_lengths=x)
+            assert float(out[0].abs().max()) == 0.0 and torch.equal(out[1], full)
 
 
 def test_nothing_to_do(C):

@@ -1,6 +1,6 @@
 // abi_asan.cpp — AddressSanitizer driver for the HOST side of libecnf_hip.so ("-fsanitize=address
 // host build").  Built by tools/asan/build.sh against an ASan-instrumented build of the host translation units
-// (ecnf_hip.hip host code, ecnf_train.hip host code); device code is not instrumented (no GPU ASan on this pool).
+// (the host code of ecnf_hip.hip, ecnf_train.hip and ecnf_context.hip); device code is not instrumented (no GPU ASan on this pool).
 //
 // Without a GPU it exercises every host path that runs before the first device call: argument checks, the
 // ravel_pytree param walk and the split / fragment repacking of ecnf_create (which then fails with ECNF_E_HIP).
@@ -201,6 +201,56 @@ static bool device_checks(const ecnf_cfg& c, int B) {
   return true;
 }
 
+// the context operators: refusals on the host; with a device also one small forward and backward pass of each
+static void context_checks(bool gpu) {
+  ecnf_qk_norm n;
+  std::memset(&n, 0, sizeof n);
+  size_t bytes = 0;
+  CHECK(ecnf_qk_norm_workspace_size(nullptr, &bytes) == ECNF_E_INVALID, "norm NULL");
+  CHECK(ecnf_qk_norm_rotary(&n, nullptr) == ECNF_E_UNSUPPORTED, "norm head_dim 0");
+  CHECK(ecnf_qk_norm_rotary_grad(&n, nullptr, 0, nullptr) == ECNF_E_UNSUPPORTED, "norm grad head_dim 0");
+  ecnf_attention a;
+  std::memset(&a, 0, sizeof a);
+  CHECK(ecnf_cross_attention_workspace_size(&a, 0, &bytes) == ECNF_E_INVALID, "attention empty");
+  CHECK(ecnf_cross_attention(&a, nullptr, 0, nullptr) == ECNF_E_INVALID, "attention empty");
+  CHECK(ecnf_cross_attention_grad(&a, nullptr, 0, nullptr) == ECNF_E_INVALID, "attention grad empty");
+  CHECK(ecnf_vector_field_nodes(nullptr, nullptr, nullptr, nullptr, 1, nullptr, nullptr, 1, nullptr) == ECNF_E_INVALID, "nodes");
+  CHECK(ecnf_integrate_nodes(nullptr, nullptr, nullptr, nullptr, 1, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, 1,
+                             nullptr, 0, nullptr) == ECNF_E_INVALID, "integrate nodes");
+  CHECK(ecnf_fm_loss_grad_nodes(nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, 0.f, 1, nullptr, nullptr, nullptr,
+                                nullptr) == ECNF_E_INVALID, "loss nodes");
+  if (!gpu) return;
+  const int B = 2, Lq = 5, Lk = 300, H = 2, D = 16;
+  float *q = dev_alloc<float>(B * Lq * H * D), *k = dev_alloc<float>(B * Lk * H * D), *o = dev_alloc<float>(B * Lq * H * D);
+  float *dq = dev_alloc<float>(B * Lq * H * D), *dk = dev_alloc<float>(B * Lk * H * D), *dv = dev_alloc<float>(B * Lk * H * D);
+  float *lse = dev_alloc<float>(B * H * Lq), *w = dev_alloc<float>(D), *dw = dev_alloc<float>(D);
+  int32_t* pos = dev_alloc<int32_t>(Lq);
+  n.q.x = q; n.q.grad = o; n.q.out = dq; n.q.weight = w; n.q.weight_grad = dw; n.q.positions = pos;
+  n.q.batch = B; n.q.length = Lq; n.q.heads = H; n.q.position_type = ECNF_POS_I32; n.q.position_stride[1] = 1;
+  for (int64_t* st : {n.q.x_stride, n.q.grad_stride, a.q_stride, a.out_grad_stride}) st[0] = Lq * H * D, st[1] = H * D, st[2] = D;
+  for (int64_t* st : {a.k_stride, a.v_stride}) st[0] = Lk * H * D, st[1] = H * D, st[2] = D;
+  n.dtype = ECNF_DTYPE_F32; n.head_dim = D; n.n_axes = 1; n.axes[0] = D; n.eps = 1e-6f; n.theta = 1e4;
+  CHECK(ecnf_qk_norm_rotary(&n, nullptr) == ECNF_OK, "norm");
+  CHECK(ecnf_qk_norm_workspace_size(&n, &bytes) == ECNF_OK && bytes > 0, "norm workspace");
+  float* ws = dev_alloc<float>(bytes / 4);
+  CHECK(ecnf_qk_norm_rotary_grad(&n, ws, bytes, nullptr) == ECNF_OK, "norm grad");
+  CHECK(ecnf_qk_norm_rotary_grad(&n, ws, bytes - 1, nullptr) == ECNF_E_INVALID, "norm grad, small workspace");
+  hipFree(ws);
+  a.q = q; a.k = k; a.v = k; a.out = o; a.out_grad = o; a.lse = lse; a.q_grad = dq; a.k_grad = dk; a.v_grad = dv;
+  a.dtype = ECNF_DTYPE_F32; a.batch = a.context_batch = B; a.n_queries = Lq; a.context_length = Lk; a.heads = a.kv_heads = H;
+  a.head_dim = D; a.scale = 0.25f;
+  for (int grad = 0; grad < 2; ++grad) {
+    CHECK(ecnf_cross_attention_workspace_size(&a, grad, &bytes) == ECNF_OK, "attention workspace");
+    ws = dev_alloc<float>(bytes / 4 + 4);
+    const int rc = grad ? ecnf_cross_attention_grad(&a, ws, bytes, nullptr) : ecnf_cross_attention(&a, ws, bytes, nullptr);
+    CHECK(rc == ECNF_OK, "attention %d", grad);
+    CHECK(hipDeviceSynchronize() == hipSuccess, "attention %d", grad);
+    hipFree(ws);
+  }
+  for (void* p : {(void*)q, (void*)k, (void*)o, (void*)dq, (void*)dk, (void*)dv, (void*)lse, (void*)w, (void*)dw, (void*)pos})
+    if (p) hipFree(p);
+}
+
 int main() {
   host_checks();
   const ecnf_cfg cfgs[] = {make_cfg(4, 2, 1, 64, 128, 3, 3, 1.f), make_cfg(13, 3, 1, 64, 128, 3, 3, 1.f),
@@ -210,6 +260,7 @@ int main() {
     if (g_trace) std::fprintf(stderr, "config N = %d, M = %d\n", c.n_nodes, c.mlp_width);
     gpu += device_checks(c, 5) ? 1 : 0;
   }
+  context_checks(gpu > 0);
   {
     size_t lay[16];
     for (int w = 0; w < 4; ++w) CHECK(ecnf_struct_layout(w, lay, 16) > 0, "struct layout %d", w);
