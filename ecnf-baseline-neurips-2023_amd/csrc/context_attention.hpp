@@ -139,41 +139,43 @@ __device__ __forceinline__ float sum_halves(float x) {
 }
 
 // The backward pass in fp16.  P is about 1 / keys and dS smaller still, at or below fp16's subnormals in long contexts
-// (1 / 16384 = 2^-14), so both are rounded as multiples of a power of two, which the accumulators carry: kPScale for P
-// (at most 1, so at most 2^14), and for dS one a column (row of dQ, key of dK), moved as the largest |dS| so far needs it.
-// What is rounded away is then 2^-12 of the value, or 2^-39 of the column's largest.
-constexpr float kPScale = 16384.f;
+// (1 / 16384 = 2^-14).  So P is made as 2^14 P (at most 2^14: a shift of the exponent's argument, for nothing), dS with
+// it, and where the largest 2^14 |dS| of a column (row of dQ, key of dK) so far is not in [1, 2^15] the column is scaled
+// by a power of two besides, which its accumulators carry.  What is rounded away is then 2^-12 of the value, or 2^-25 of
+// the column's largest.  Other types have fp32's exponents and need nothing.
 template <class T>
-struct Range {   // types with fp32's exponents need nothing
+struct Range {
+  static constexpr float kShift = 0.f, kBack = 1.f;
   __device__ __forceinline__ void fit(f32x16&, f32x16*, int) {}
   __device__ __forceinline__ float back() const { return 1.f; }
-  static constexpr float kP = 1.f;
 };
 template <>
 struct Range<_Float16> {
-  static constexpr float kP = kPScale;
-  float scale = 0x1p120f;
+  static constexpr float kShift = 14.f, kBack = 0x1p-14f;
+  float scale = 1.f, top = 0.f;
   // scales x (one column a lane, its other rows in the other half), and the accumulators where the scale moves
   __device__ __forceinline__ void fit(f32x16& x, f32x16* acc, int n) {
     float m = 0.f;
 #pragma unroll
     for (int i = 0; i < 16; ++i) m = fmaxf(m, fabsf(x[i]));
-    m = max_halves(m);
-    if (__any(m * scale > 32768.f)) {
+    top = fmaxf(top, max_halves(m));
+    const float at = top * scale;
+    const bool out = at > 32768.f || (at < 1.f && at > 0.f);
+    if (__any(out)) {
       // the largest lands in [2^14, 2^15); an infinity or NaN stays one
-      const int e = (int)(__float_as_uint(m) >> 23);
-      const float want = __uint_as_float((uint32_t)min(max(268 - e, 1), 254) << 23);
-      const float next = fminf(scale, want), move = next / scale;
+      const uint32_t e = (uint32_t)min(max(268 - (int)(__float_as_uint(top) >> 23), 1), 254);
+      const float next = out ? __uint_as_float(e << 23) : scale, move = next / scale;
       scale = next;
 #pragma unroll
       for (int d = 0; d < n; ++d)
 #pragma unroll
         for (int i = 0; i < 16; ++i) acc[d][i] *= move;
     }
+    if (__any(scale != 1.f))
 #pragma unroll
-    for (int i = 0; i < 16; ++i) x[i] *= scale;
+      for (int i = 0; i < 16; ++i) x[i] *= scale;
   }
-  __device__ __forceinline__ float back() const { return 1.f / scale; }
+  __device__ __forceinline__ float back() const { return kBack / scale; }
 };
 
 // A row-major tile in LDS, rows of DP elements, its 16-byte chunks swizzled inside a row: chunk c of row r sits at
@@ -765,7 +767,8 @@ __global__ __launch_bounds__(256) ECNF_WAVES(waves(HD, sizeof(T), 4, 3)) void at
   f32x16 acc[ND];
 #pragma unroll
   for (int d = 0; d < ND; ++d) acc[d] = f32x16{};
-  // P and dP of the 32 keys from k0 of the tile at kat, vat
+  const float shift = Range<T>::kShift - lse;
+  // P (2^kShift of it) and dP of the 32 keys from k0 of the tile at kat, vat
   auto products = [&](int t, uint32_t kat, uint32_t vat, int k0, f32x16& p, f32x16& dp) __attribute__((always_inline)) {
     p = f32x16{}, dp = f32x16{};
 #pragma unroll
@@ -783,7 +786,7 @@ __global__ __launch_bounds__(256) ECNF_WAVES(waves(HD, sizeof(T), 4, 3)) void at
       }
     }
 #pragma unroll
-    for (int x = 0; x < 16; ++x) p[x] = __builtin_amdgcn_exp2f(fmaf(p[x], sc, -lse));
+    for (int x = 0; x < 16; ++x) p[x] = __builtin_amdgcn_exp2f(fmaf(p[x], sc, shift));
   };
   ks.start();
   // A context of one tile: delta = sum_j P dP over its keys instead of sum_d dO O.  With few keys dP - delta cancels,
@@ -804,7 +807,7 @@ __global__ __launch_bounds__(256) ECNF_WAVES(waves(HD, sizeof(T), 4, 3)) void at
 #pragma unroll
         for (int x = 0; x < 16; ++x) sum = fmaf(p[x], dp[x], sum);
       }
-    sum = sum_halves(sum);
+    sum = sum_halves(sum) * Range<T>::kBack;
     if constexpr (WK == 1) {
       delta = sum;
     } else {
@@ -850,7 +853,7 @@ __global__ __launch_bounds__(256) ECNF_WAVES(waves(HD, sizeof(T), 4, 3)) void at
     if (Sh::kBufs == 2 && t + 1 < ks.t1) step(t + 1, Const<1>{});
   }
 
-  if constexpr (Range<T>::kP != 1.f) {
+  if constexpr (Range<T>::kShift != 0.f) {
     const float back = range.back();
 #pragma unroll
     for (int d = 0; d < ND; ++d) acc[d] *= back;
@@ -993,7 +996,7 @@ __global__ __launch_bounds__(256) ECNF_WAVES(waves(HD, sizeof(T), 3, 2)) void at
     }
   };
   auto publish = [&](int buf) {
-    if (tid < kRows) stats[buf * 2 * kRows + tid] = nl, stats[(buf * 2 + 1) * kRows + tid] = nd;
+    if (tid < kRows) stats[buf * 2 * kRows + tid] = nl - Range<T>::kShift, stats[(buf * 2 + 1) * kRows + tid] = nd;
   };
   if (t0 < t1) {
     fetch(t0, 0);
@@ -1027,7 +1030,7 @@ __global__ __launch_bounds__(256) ECNF_WAVES(waves(HD, sizeof(T), 3, 2)) void at
         for (int x = 0; x < 4; ++x) {
           float p = __builtin_amdgcn_exp2f(fmaf(sx[4 * j + x], sc, -ls[x]));
           p = ok ? p : 0.f;
-          sx[4 * j + x] = p * Range<T>::kP;
+          sx[4 * j + x] = p;
           dp[4 * j + x] = p * (dp[4 * j + x] - de[x]);
         }
       }
@@ -1051,10 +1054,10 @@ __global__ __launch_bounds__(256) ECNF_WAVES(waves(HD, sizeof(T), 3, 2)) void at
     }
   }
 
-  if constexpr (Range<T>::kP != 1.f) {
+  if constexpr (Range<T>::kShift != 0.f) {
     const float back = range.back();
 #pragma unroll
-    for (int d = 0; d < ND; ++d) dk[d] *= back, dv[d] *= 1.f / kPScale;
+    for (int d = 0; d < ND; ++d) dk[d] *= back, dv[d] *= Range<T>::kBack;
   }
   const int64_t n_keys = (int64_t)a.C * a.Hk * a.Lk;
   auto put = [&](int which, int kk, int d, f32x4 v) {

@@ -77,13 +77,13 @@ def attention(q, k, v, query_lengths=None, context_lengths=None, context_mask=No
     eP = eP + 2 * t_lse
     t_delta = (G.abs() * (tO + D * E * O.abs())).sum(-1, keepdim=True)
     t_dP = (D + 2) * E * (G.abs() @ V.abs().transpose(2, 3))
-    # fp16: what a column's scale cuts off is 2^-39 of its largest dS
-    cut = 2.0 ** -39 if q.dtype == torch.float16 else 0.0
+    # fp16: what a column's scale cuts off is 2^-25 of its largest dS, and of 2^14 P 2^-25
+    cut = 2.0 ** -25 if q.dtype == torch.float16 else 0.0
     tS = (up + eP + 4 * E) * dS.abs() + P * (t_dP + t_delta) + cut * (dS.abs().amax((2, 3), keepdim=True) if Lk else 0.0)
     n = Q.shape[2]
     tQ = abs(scale) * (tS + (Lk + 2) * E * dS.abs()) @ K.abs()
     tK = abs(scale) * (tS + (n + 2) * E * dS.abs()).transpose(2, 3) @ Q.abs()
-    tV = ((up + eP + (n + 2) * E) * P + cut * (P > 0)).transpose(2, 3) @ G.abs()
+    tV = ((up + eP + (n + 2) * E) * P + cut * 2.0 ** -14 * (P > 0)).transpose(2, 3) @ G.abs()
     dQ, dK, dV = scale * dS @ K, scale * dS.transpose(2, 3) @ Q, P.transpose(2, 3) @ G
     res["dq"] = (back(dQ), back(tQ + u * dQ.abs() + d))
     res["dk"] = tuple(x.permute(0, 2, 1, 3) for x in (dK, tK + u * dK.abs() + d))
