@@ -858,6 +858,9 @@ __global__ __launch_bounds__(256) ECNF_WAVES(waves(HD, sizeof(T), 4, 3)) void at
 #pragma unroll
     for (int d = 0; d < ND; ++d) acc[d] *= back;
   }
+  if (lse == kInf)   // a row without keys: 0, also where its dO is NaN
+#pragma unroll
+    for (int d = 0; d < ND; ++d) acc[d] = f32x16{};
   const int64_t n_rows = (int64_t)a.C * a.Hk * a.R, row0 = ((int64_t)c * a.Hk + hk) * a.R;
   auto put = [&](int rr, bool lv, int bb, int ii, int gg, int d, f32x4 v) {
     if (rr >= a.R) return;
@@ -1059,6 +1062,9 @@ __global__ __launch_bounds__(256) ECNF_WAVES(waves(HD, sizeof(T), 3, 2)) void at
 #pragma unroll
     for (int d = 0; d < ND; ++d) dk[d] *= back, dv[d] *= Range<T>::kBack;
   }
+  if (!ok)   // a key that no row may read: 0, also where a dO is NaN
+#pragma unroll
+    for (int d = 0; d < ND; ++d) dk[d] = dv[d] = f32x16{};
   const int64_t n_keys = (int64_t)a.C * a.Hk * a.Lk;
   auto put = [&](int which, int kk, int d, f32x4 v) {
     if (kk >= a.Lk || d >= a.D) return;

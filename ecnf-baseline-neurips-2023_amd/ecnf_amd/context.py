@@ -71,6 +71,13 @@ def _stream(device: torch.device) -> int:
     return torch._C._cuda_getCurrentRawStream(device.index)
 
 
+def _pack(layout: struct.Struct, *values) -> bytes:
+    try:
+        return layout.pack(*values)
+    except struct.error as e:
+        raise ValueError(f"a size or axis is out of its 32-bit range ({e})") from None
+
+
 def _new(x: torch.Tensor) -> torch.Tensor:
     return torch.empty_like(x, memory_format=_CONTIGUOUS)
 
@@ -129,8 +136,8 @@ def _norm_call(q, k, axes, theta, eps, interleaved, grad: bool):
         keep.append((w32, p))   # alive until the launch
     x = q[0]
     device = x.device
-    args = _QK_NORM.pack(*packed, _DTYPES[x.dtype], x.shape[3], n_axes, *(axes + _NO_AXES)[:4], bool(interleaved),
-                         device.index, eps, theta)
+    args = _pack(_QK_NORM, *packed, _DTYPES[x.dtype], x.shape[3], n_axes, *(axes + _NO_AXES)[:4], bool(interleaved),
+                 device.index, eps, theta)
     lib = _lib.load()
     if not grad:
         _lib.check(lib.ecnf_qk_norm_rotary(args, _stream(device)))
@@ -224,10 +231,10 @@ def _attention_args(q, k, v, out, dout, lse, dq, dk, dv, ql, cl, m, scale) -> by
 
     def ptr(t):
         return 0 if t is None else t.data_ptr()
-    return _ATTENTION.pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), ptr(dout), ptr(lse), ptr(dq), ptr(dk),
-                           ptr(dv), ptr(ql), ptr(cl), ptr(m), *_strides(q), *_strides(k), *_strides(v),
-                           *(_NO_STRIDES if dout is None else _strides(dout)), _DTYPES[q.dtype], B, C, Lq, Lk, Hq, Hk, D,
-                           q.device.index, scale)
+    return _pack(_ATTENTION, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), ptr(dout), ptr(lse), ptr(dq), ptr(dk),
+                 ptr(dv), ptr(ql), ptr(cl), ptr(m), *_strides(q), *_strides(k), *_strides(v),
+                 *(_NO_STRIDES if dout is None else _strides(dout)), _DTYPES[q.dtype], B, C, Lq, Lk, Hq, Hk, D,
+                 q.device.index, scale)
 
 
 def _run_attention(args: bytes, grad: int, device) -> None:
@@ -331,6 +338,7 @@ def _project(x: torch.Tensor, w: torch.Tensor, heads: int) -> torch.Tensor:
     return (x.reshape(-1, x.shape[-1]) @ w.to(x.dtype)).reshape(x.shape[0], x.shape[1], heads, -1)
 
 
+@torch.no_grad()
 def node_embedding(embedding: torch.Tensor, features, context: Context, cnf_cfg: CNFConfig,
                    return_saved: bool = False):
     """h_i = E[f_i] + W_out attention(norm_rotary(W_q E[f_i]), norm_rotary(W_k s), W_v s) for every atom i:
@@ -374,6 +382,7 @@ def node_embedding(embedding: torch.Tensor, features, context: Context, cnf_cfg:
     return nodes, (f, x, s, q, k, v, qr, kr, o, lse, turn, keep, p, embedding.shape)
 
 
+@torch.no_grad()
 def node_embedding_grad(d_nodes: torch.Tensor, saved) -> Dict[str, torch.Tensor]:
     """Gradients of :func:`node_embedding` for the gradient of its result: {"embedding" (the table's), "states", and one
     per context parameter}, each in its operand's dtype."""

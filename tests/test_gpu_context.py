@@ -413,6 +413,59 @@ def test_nan_in_a_row_stays_in_the_row(C):
     assert torch.equal(out[keep], want[keep])
 
 
+@pytest.mark.parametrize("dtype", TYPES, ids=ids)
+@pytest.mark.parametrize("rows,keys", [(5, 40), (200, 40), (5, 700), (200, 300)])
+def test_nan_gradients_stay_with_their_row(C, dtype, rows, keys):
+    """NaN in out_grad: 0 for a row without keys and for keys that no row may read, and the rows beside it as they were."""
+    g = gen(13)
+    q, do = normal(g, 2, rows, 2, 32, dtype=dtype), normal(g, 2, rows, 2, 32, dtype=dtype)
+    k, v = normal(g, 2, keys, 1, 32, dtype=dtype), normal(g, 2, keys, 1, 32, dtype=dtype)
+    mask = torch.ones((2, keys), dtype=torch.bool, device="cuda")
+    mask[0] = False                                    # no row of molecule 0 has a key
+    mask[1, ::3] = False
+    out, lse = C.cross_attention(q, k, v, context_mask=mask, return_lse=True)
+    want = C.cross_attention_grad(do, q, k, v, out, lse, context_mask=mask)[0]
+    do[:, 3, 1] = math.nan
+    dq, dk, dv = C.cross_attention_grad(do, q, k, v, out, lse, context_mask=mask)
+    assert float(dq[0].abs().max()) == 0.0
+    for x in (dk, dv):
+        assert float(x[~mask].abs().max()) == 0.0
+        assert bool(torch.isnan(x[mask]).all())
+    assert bool(torch.isnan(dq[1, 3, 1]).all())
+    dq[1, 3, 1] = want[1, 3, 1]
+    assert torch.equal(dq, want)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=ids)
+def test_offsets_past_32_bits(C, dtype):
+    """Rows of k, v and q far apart (more than 2^32 bytes from the first to the last): as their contiguous copies."""
+    g, e = gen(14), torch.finfo(dtype).bits // 8
+    step = (8 << 20) // e - 64                         # elements from one key to the next (the largest is below 8 MiB)
+    far = torch.empty(620 * step, dtype=dtype, device="cuda")
+    k = far.as_strided((1, 620, 1, 32), (step, step, 32, 1))
+    v = far.as_strided((1, 620, 1, 32), (step, step, 32, 1), 32)
+    q = far.as_strided((2, 40, 1, 32), (300 * step, 7 * step, 32, 1), 64)
+    do = far.as_strided((2, 40, 1, 32), (300 * step, 7 * step, 32, 1), 96)
+    for x in (k, v, q, do):
+        x.copy_(normal(g, *x.shape, dtype=dtype))
+    near = [x.contiguous() for x in (q, k, v, do)]
+    pq, pk = torch.arange(40, device="cuda")[:, None], torch.arange(620, device="cuda")[:, None]
+    turn = dict(q_positions=pq, k_positions=pk, axes=(32,))
+
+    def run(q, k, v, do):
+        o = C.cross_attention(q, k, v, return_lse=True)
+        return (*o, *C.cross_attention_grad(do, q, k, v, *o), *C.qk_norm_rotary(q, k, **turn),
+                *C.qk_norm_rotary_grad(do, v, q, k, **turn)[:2])
+    for a, b in zip(run(q, k, v, do), run(*near)):
+        assert torch.equal(a, b)
+
+
+def test_sizes_out_of_their_range(C):
+    x, p = normal(gen(0), 1, 4, 1, 16), torch.zeros((4, 1), device="cuda")
+    with pytest.raises(ValueError, match="32-bit"):
+        C.qk_norm_rotary(x, q_positions=p, axes=(2 ** 40,))
+
+
 def test_rows_behind_the_outputs_are_left_alone():
     """The C entry writes its outputs and nothing behind them."""
     import ctypes

@@ -179,6 +179,17 @@ def test_node_embedding_and_its_gradients(contexts, length):
         assert float((got[n] - w).abs().max()) <= tol * max(float(w.abs().max()), uncancelled), n
 
 
+def test_results_carry_no_autograd_history():
+    """Leaves that require gradients: the results have none of their own (a part of the chain would be worse than none)."""
+    cfg = CONFIGS["aldp"]
+    ctx = make_context(cfg, 1, 20)
+    table = torch.randn((cfg.n_features, cfg.hidden), device="cuda", requires_grad=True)
+    ctx = ctx._replace(params={n: p.requires_grad_() for n, p in ctx.params.items()})
+    nodes, saved = C.node_embedding(table, features(cfg), ctx, cfg, return_saved=True)
+    grads = C.node_embedding_grad(torch.ones_like(nodes), saved)
+    assert not nodes.requires_grad and not any(x.requires_grad for x in grads.values())
+
+
 def test_shared_features_and_context_are_computed_once():
     cfg = CONFIGS["aldp"]
     ctx = make_context(cfg, 1, 20)
