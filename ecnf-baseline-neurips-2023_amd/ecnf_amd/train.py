@@ -272,11 +272,13 @@ def flow_matching_loss_fn(cnf, params, x_data, key, features=None, *, x0=None, t
 
 
 def flow_matching_update_fn(cnf, opt: Adam, state: TrainingState, x_data, features=None, ema_beta: float = 0.999,
-                            *, x0=None, t=None):
+                            *, x0=None, t=None, context=None):
     """gradient_step.py:21-53: grads of the flow-matching loss, one Adam step, optional EMA; returns
-    (new TrainingState, info{loss, grad_norm, update_norm})."""
+    (new TrainingState, info{loss, grad_norm, update_norm}).  context: as in :func:`flow_matching_loss_fn`; its own
+    parameters are the caller's to step, by info["context_grad"]."""
     g = _generator(state.key, cnf.device)
-    loss, info, grad = flow_matching_loss_fn(cnf, state.params, x_data, g, features, x0=x0, t=t, with_grad=True)
+    loss, info, grad = flow_matching_loss_fn(cnf, state.params, x_data, g, features, x0=x0, t=t, with_grad=True,
+                                             context=context)
     tr = trainer_for(cnf.cfg, int(torch.as_tensor(x_data).shape[0]), cnf.device)
     params = state.params.clone()
     mu, nu = state.opt_state.mu.clone(), state.opt_state.nu.clone()

@@ -294,6 +294,29 @@ def test_loss_gradient(name, contexts):
     assert torch.equal(grad, grad2) and all(torch.equal(cg[k], info2["context_grad"][k]) for k in cg)
 
 
+def test_update_step():
+    """flow_matching_update_fn with a context: the loss and gradients of flow_matching_loss_fn, Adam on the field's."""
+    cnf = build("lj13")
+    cfg = cnf.cfg
+    g = torch.Generator(device="cuda")
+    g.manual_seed(7)
+    B = 5
+    x1, x0 = cnf.sample_base(g, B) * 1.5, cnf.sample_base(g, B)
+    t = torch.rand(B, generator=g, device="cuda")
+    f = features(cfg)[None].expand(B, -1).contiguous()
+    ctx = make_context(cfg, 1, 25)
+    params = torch.as_tensor(F.flatten_params(init_params(cfg, 6), cfg), device="cuda")
+    loss, want, grad = TR.flow_matching_loss_fn(cnf, params, x1, None, f, x0=x0, t=t, with_grad=True, context=ctx)
+    opt = TR.adam(1e-3)
+    state = TR.init_training_state(cnf, params, opt, key=0)
+    new, info = TR.flow_matching_update_fn(cnf, opt, state, x1, f, x0=x0, t=t, context=ctx)
+    assert torch.equal(info["loss"], loss)
+    assert all(torch.equal(info["context_grad"][n], want["context_grad"][n]) for n in want["context_grad"])
+    moved = params - new.params                        # Adam's first step: lr * grad / (|grad| + eps)
+    at = grad.abs() > 1e-4 * grad.abs().max()
+    assert torch.equal(moved[at].sign(), grad[at].sign())
+
+
 def test_padded_widths():
     """A reference network zero-padded onto a compiled shape: embeddings of the reference's width, same results as ids."""
     cnf = F.build_cnf(n_frames=5, dim=3, sigma_min=0.01, base_scale=1.0, n_blocks_egnn=2, mlp_units=(48, 40),
