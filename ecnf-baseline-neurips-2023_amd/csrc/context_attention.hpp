@@ -80,6 +80,7 @@ struct Att {
   int32_t R;                       // rows of a (context, key head): per * Lq * G
   int32_t tiles;                   // row or key tiles of a (context, key head)
   int32_t splits;
+  int32_t elem;                    // bytes of an element
   int32_t flat;                    // tokens of a context are one sequence in q and dout (see RowTile)
   float scale;
 };
@@ -409,6 +410,13 @@ __device__ __forceinline__ void store4(char* p, f32x4 v) {
 // forward.  A workgroup of 4 waves: WR of them split the rows (32 each), WK the keys of a tile (KT each); the waves of
 // one row block join their statistics and outputs through LDS at the end.  grid = contexts * key heads * tiles * splits;
 // with splits > 1 a workgroup takes its share of the key tiles and leaves a normalised fp32 partial and its lse.
+//
+// Long contexts are bound by the matrix units and the exponentials beside them (MFMA busy 0.51, vector 0.46 of a clock
+// that falls to 1.83 GHz; no LDS bank conflict): 2 x 4096 queries of 32 heads on 8192 keys of 8, 128 wide, bf16, 1037 us,
+// 1060 TFLOP/s (a library product of 8192^3: 1163).  So 32 rows a wave, tiles of 64 keys in two buffers with one barrier
+// each; 64 rows a wave spill (1341 us), tiles of 32 pay the barrier twice (1106).  Single tokens are bound by reading
+// K and V: 64 x 8192 keys of 8 x 128 in 376 us, 5.7 TB/s.  Small contexts by latency: 512 x 22 rows x 333 masked keys of
+// 4 x 64, bf16, 30 us, 3.6 TB/s.
 // ---------------------------------------------------------------------------------------------------------------
 template <class T, int DP, int WR, int WK, int KT, int BUFS>
 struct FwdShape {
@@ -675,7 +683,8 @@ __global__ __launch_bounds__(256) ECNF_WAVES(waves(HD, sizeof(T), 4, 4)) void at
   }
 }
 
-// joins the splits of the forward pass: out = sum_s 2^(lse_s - M) part_s / sum_s 2^(lse_s - M); a thread has 4 columns
+// joins the splits of the forward pass: out = sum_s 2^(lse_s - M) part_s / sum_s 2^(lse_s - M); a thread has 4 columns.
+// Its loads are in flight together (one by one, 64 splits of 32 rows took 20 us of a 151 us call).
 template <class T>
 __global__ __launch_bounds__(256) void att_fwd_join(Att a) {
   const int64_t n = (int64_t)a.C * a.Hk * a.R;
@@ -685,10 +694,12 @@ __global__ __launch_bounds__(256) void att_fwd_join(Att a) {
   if (row >= n) return;
   const int ch = (int)(x - row * D4);
   float M = -kInf;
+#pragma unroll 16
   for (int s = 0; s < a.splits; ++s) M = fmaxf(M, a.part_lse[s * n + row]);
   const float ref = M == -kInf ? 0.f : M;
   float L = 0.f;
   f32x4 v = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 16
   for (int s = 0; s < a.splits; ++s) {
     const float e = __builtin_amdgcn_exp2f(a.part_lse[s * n + row] - ref);
     L += e;
@@ -712,6 +723,10 @@ __global__ __launch_bounds__(256) void att_fwd_join(Att a) {
 // transposed layout, so P and dS need one lse and one delta a lane, and dQ^T += K^T dS^T takes dS from its accumulator
 // registers.  Also writes every row's delta and lse (log2 units; +inf for a row without keys, whose P is then 0) for
 // the kernel below.
+//
+// Bound by the matrix units (busy 0.55 of 1.9 GHz, vector 0.37): 4096 queries of 32 heads on 8192 keys of 8, 128 wide,
+// bf16, 745 us, 1107 TFLOP/s of its three products; 22 x 129 in fp32, 2048 times, 20 us, by latency (four short phases a
+// workgroup).
 // ---------------------------------------------------------------------------------------------------------------
 template <class T, int HD, int WR, int WK, int KT, int BUFS>
 __global__ __launch_bounds__(256) ECNF_WAVES(waves(HD, sizeof(T), 4, 3)) void att_dq(Att a) {
@@ -908,6 +923,11 @@ __global__ __launch_bounds__(256) ECNF_WAVES(waves(HD, sizeof(T), 4, 3)) void at
 // pass through LDS.  S and dP have keys across, so P and dS are the B operands of dV^T += dO^T P and dK^T += Q^T dS as
 // they stand.  WY waves split the keys of a workgroup, WX its rows (joined through LDS); with splits > 1 a workgroup
 // takes its share of the row tiles and leaves fp32 partials.  The order of every sum is fixed.
+//
+// Bound by the matrix units and, at 128, by the registers: two gradients of 32 keys take half of them, which leaves two
+// waves a SIMD and few reads ahead (MFMA busy 0.45, vector 0.35, LDS 0.34; 2.1 GHz).  4096 queries of 32 heads on 8192
+// keys of 8, 128 wide, bf16: 1100 us, 1000 TFLOP/s of its four products; with V in registers too 1425.  22 rows x 129
+// keys in fp32, 2048 times: 39 us, by latency; the last of a context's five key blocks has a workgroup of its own.
 // ---------------------------------------------------------------------------------------------------------------
 template <class T, int DP, int WY, int WX>
 struct DkvShape {
@@ -1108,7 +1128,8 @@ __global__ __launch_bounds__(256) ECNF_WAVES(waves(HD, sizeof(T), 3, 2)) void at
   }
 }
 
-// sums the splits' partials (in order): which = 0 dQ rows, 1 dK and dV keys (blockIdx.y: 0 dK, 1 dV); 4 columns a thread
+// sums the splits' partials (in order): which = 0 dQ rows, 1 dK and dV keys (blockIdx.y: 0 dK, 1 dV); 4 columns a thread.
+// 16 splits of 512 keys of 8 x 64 (fp16 gradients): 8 us, most of it start and end.
 template <class T>
 __global__ __launch_bounds__(256) void att_grad_join(Att a, int which) {
   const int D4 = a.D / 4;
@@ -1119,6 +1140,7 @@ __global__ __launch_bounds__(256) void att_grad_join(Att a, int which) {
   const int d = 4 * (int)(x - row * D4);
   const int kinds = which ? 2 : 1, y = which ? (int)blockIdx.y : 0;
   f32x4 v = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 16
   for (int s = 0; s < a.splits; ++s)
     v += *reinterpret_cast<const f32x4*>(a.part + (((int64_t)s * kinds + y) * n + row) * a.D + d);
   const int len = which ? a.Lk : a.R;
@@ -1150,16 +1172,26 @@ struct Plan {
 
 inline int ceil_div(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
 
-// outer: rows (forward, dQ) or keys (dK dV) of a (context, key head); inner: the loop's length, and its tiles'; per_row: partial floats of one outer element and split.
-inline Plan make_plan(int64_t pairs, int outer, int inner, int narrow_step, int wide_step, int64_t per_row, bool lse) {
+// outer: rows (forward, dQ) or keys (dK dV) of a (context, key head); inner: the loop's length, and its tiles';
+// per_row: partial floats of one outer element and split.
+//
+// The loop is split until the workgroups fill the chip once (one a CU where a row of a tile has 256 bytes or more: their
+// buffers fill its LDS; else two), but into parts of no fewer than 2 tiles (narrow), 8 (16-bit types) or 4 (fp32, whose
+// tiles take longer).  Measured, us: one token, 131072 keys of 8 x 128, bf16: one a CU 111, two 129; gradients of 22 x 1024
+// rows on 512 keys of 8 x 64, fp16: 162, two 138; 22 fp32 rows on 4 x 4096 keys of 4 x 32: parts of 4 tiles 31, of 2 27;
+// gradients of 100 rows on 2 x 4000 keys of 4 x 64, bf16: parts of 4 tiles 56, of 8 40; 300 fp32 rows on 2000 keys: 52
+// and 71.
+inline Plan make_plan(const Att& a, int outer, int inner, int narrow_step, int wide_step, int64_t per_row, bool lse) {
   Plan p;
+  const int64_t pairs = (int64_t)a.C * a.Hk;
   p.narrow = outer <= 32;
   p.tiles = ceil_div(outer, p.narrow ? 32 : 128);
   const int64_t base = pairs * p.tiles;
+  const int fill = tile_width(a.D) * a.elem > 128 ? 256 : 512, least = p.narrow ? 2 : a.elem == 4 ? 4 : 8;
   const int inner_tiles = ceil_div(inner, p.narrow ? narrow_step : wide_step);
   int64_t s = 1;
-  if (base > 0 && base < 512) s = (512 + base - 1) / base;
-  if (s > inner_tiles / 4) s = inner_tiles / 4;
+  if (base > 0 && base < fill) s = (fill + base - 1) / base;
+  if (s > inner_tiles / least) s = inner_tiles / least;
   const int64_t one = pairs * outer * per_row;
   if (one > 0 && s * one > kPartMax) s = kPartMax / one;
   p.splits = (int)(s < 1 ? 1 : s);
@@ -1169,9 +1201,9 @@ inline Plan make_plan(int64_t pairs, int outer, int inner, int narrow_step, int 
   p.part_lse = p.splits > 1 && lse ? (int64_t)p.splits * pairs * outer : 0;
   return p;
 }
-inline Plan plan_fwd(const Att& a) { return make_plan((int64_t)a.C * a.Hk, a.R, a.Lk, 128, 64, a.D, true); }
-inline Plan plan_dq(const Att& a) { return make_plan((int64_t)a.C * a.Hk, a.R, a.Lk, 128, 64, a.D, false); }
-inline Plan plan_dkv(const Att& a) { return make_plan((int64_t)a.C * a.Hk, a.Lk, a.R, 128, 32, 2 * a.D, false); }
+inline Plan plan_fwd(const Att& a) { return make_plan(a, a.R, a.Lk, 128, 64, a.D, true); }
+inline Plan plan_dq(const Att& a) { return make_plan(a, a.R, a.Lk, 128, 64, a.D, false); }
+inline Plan plan_dkv(const Att& a) { return make_plan(a, a.Lk, a.R, 128, 32, 2 * a.D, false); }
 
 // one per element type (ecnf_attention.hip)
 hipError_t launch_fwd_bf16(const Att&, hipStream_t);
