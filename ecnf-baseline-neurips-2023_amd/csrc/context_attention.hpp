@@ -792,6 +792,7 @@ __global__ __launch_bounds__(256) ECNF_WAVES(waves(HD, sizeof(T), 4, 3)) void at
       dp = Ops<T>::mma(rd.frag(vat, k0, s), df[s], dp);
     }
     if (!ks.whole(t)) {
+      if (ks.n == 1) dp *= 0.f;
       const float* bias = ks.bias();
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
@@ -834,6 +835,8 @@ __global__ __launch_bounds__(256) ECNF_WAVES(waves(HD, sizeof(T), 4, 3)) void at
       for (int k = 0; k < WK; ++k) delta += part[(k * WR + wr) * 32 + (l & 31)];
     }
   }
+  // one key: P is 1 whatever q and k are, so dS is 0 and not what dP and delta differ by
+  if (ks.n == 1) delta *= 0.f;
   if (split == 0 && wk == 0 && h == 0 && r < a.R) {
     const int64_t row = ((int64_t)c * a.Hk + hk) * a.R + r;
     a.row_lse[row] = lse;
@@ -978,9 +981,10 @@ __global__ __launch_bounds__(256) ECNF_WAVES(waves(HD, sizeof(T), 3, 2)) void at
   const int n = key_count(a, c);
   const int key = (tile * WY + wy) * 32 + (l & 31);
   const uint8_t* mask = a.mask ? a.mask + (int64_t)c * a.Lk : nullptr;
+  // (a context of one key has dP = delta = 0, as in dQ: V, which only dP reads, is taken as 0)
   const bool ok = key < n && (!mask || mask[key]);
   const char* krow = ok ? a.k + ((int64_t)c * a.ks[0] + (int64_t)key * a.ks[1] + (int64_t)hk * a.ks[2]) * e : nullptr;
-  const char* vrow = ok ? a.v + ((int64_t)c * a.vs[0] + (int64_t)key * a.vs[1] + (int64_t)hk * a.vs[2]) * e : nullptr;
+  const char* vrow = ok && n > 1 ? a.v + ((int64_t)c * a.vs[0] + (int64_t)key * a.vs[1] + (int64_t)hk * a.vs[2]) * e : nullptr;
   const uint32_t lds0 = lds_address(lds);
   Reader<T, DP> rdr;
   rdr.init(lds0, l);

@@ -255,6 +255,24 @@ def test_attention_one_key(C):
             O.check(name, got, *want[name])
 
 
+@pytest.mark.parametrize("dtype", TYPES, ids=ids)
+@pytest.mark.parametrize("rows,Lk", [(3, 1), (200, 1), (200, 70), (3, 600)])
+def test_attention_one_key_has_no_score_gradient(C, dtype, rows, Lk):
+    """A context of one key: P is 1 whatever q and k are, so dq and dk are 0 exactly, and dv is the sum of out_grad."""
+    g = gen(25)
+    q, do = normal(g, 3, rows, 4, 64, dtype=dtype), normal(g, 3, rows, 4, 64, dtype=dtype)
+    k, v = 3 * normal(g, 3, Lk, 4, 64, dtype=dtype), normal(g, 3, Lk, 4, 64, dtype=dtype)
+    n = torch.ones(3, dtype=torch.int32, device="cuda")
+    out, lse = C.cross_attention(q, k, v, context_lengths=n, return_lse=True)
+    dq, dk, dv = C.cross_attention_grad(do, q, k, v, out, lse, context_lengths=n)
+    assert float(dq.abs().max()) == 0.0 and float(dk.abs().max()) == 0.0
+    # P = 2^(s - lse) and lse, natural log, round at |s|: |P - 1| <= 2^-21 |s|; rows * 2^-23 for the sums
+    want, size = do.double().sum(1), do.double().abs().sum(1)
+    s = float(lse.abs().max())
+    tol = (2.0 ** -21 * s + rows * 2.0 ** -23 + torch.finfo(dtype).eps) * size
+    assert bool(((dv[:, 0].double() - want).abs() <= tol).all()) and float(dv[:, 1:].abs().sum()) == 0.0
+
+
 def test_attention_sharp_scores(C):
     """Scores far apart: one key takes everything, in a tile that comes late (the running maximum moves every tile)."""
     q = torch.full((1, 2, 1, 32), 2.0, device="cuda")
