@@ -385,19 +385,28 @@ def node_embedding(embedding: torch.Tensor, features, context: Context, cnf_cfg:
 @torch.no_grad()
 def node_embedding_grad(d_nodes: torch.Tensor, saved) -> Dict[str, torch.Tensor]:
     """Gradients of :func:`node_embedding` for the gradient of its result: {"embedding" (the table's), "states", and one
-    per context parameter}, each in its operand's dtype."""
+    per context parameter}: the table's in fp32, the others' in their operand's dtype, but in fp32 where that is float16
+    (a mean loss's gradients are 1e-8 and less, nothing in float16)."""
     f, x, s, q, k, v, qr, kr, o, lse, turn, keep, p, table = saved
     rows = lambda t: t.reshape(t.shape[0] * t.shape[1], -1)                 # noqa: E731
     d_nodes = d_nodes.float().reshape(x.shape)
-    dn = rows(d_nodes).to(o.dtype)
-    do = (dn @ p["out"].to(o.dtype).t()).reshape(o.shape)
-    dqr, dkr, dv = cross_attention_grad(do, qr, kr, v, o, lse, **keep)
+    weight = lambda n: p[n].to(s.dtype).float()   # what the forward pass multiplied by                   # noqa: E731
+    do = (rows(d_nodes) @ weight("out").t()).reshape(o.shape)
+    if s.dtype == torch.float16:
+        # fp16 ends at 2^-24, and the loss's mean over the batch puts these gradients below (LJ13, 1024 molecules: rms
+        # 6e-9).  No power of two is safe for all of the chain, since dK and dV are sums over the batch and the norm divides
+        # dK by the keys' size: so the operators' gradients of fp16 values are taken in fp32
+        q, k, v, qr, kr, o = (t.float() for t in (q, k, v, qr, kr, o))
+    turn = dict(turn, q_weight=turn["q_weight"].float(), k_weight=turn["k_weight"].float())   # their gradients in fp32
+    dqr, dkr, dv = cross_attention_grad(do.to(o.dtype), qr, kr, v, o, lse, **keep)
     dq, dk, dqn, dkn = qk_norm_rotary_grad(dqr, dkr, q, k, **turn)
-    g = {"query": rows(x).t() @ rows(dq), "key": rows(s).t() @ rows(dk), "value": rows(s).t() @ rows(dv),
-         "out": rows(o).t() @ dn, "query_norm": dqn, "key_norm": dkn}
-    g = {n: t.to(p[n].dtype) for n, t in g.items()}
-    g["states"] = (rows(dk) @ p["key"].to(s.dtype).t() + rows(dv) @ p["value"].to(s.dtype).t()).reshape(s.shape)
-    de = d_nodes + (rows(dq) @ p["query"].to(x.dtype).t()).float().reshape(x.shape)
+    x, st, on = (t.to(q.dtype) for t in (x, s, o))
+    g = {"query": rows(x).t() @ rows(dq), "key": rows(st).t() @ rows(dk), "value": rows(st).t() @ rows(dv),
+         "out": rows(on).t() @ rows(d_nodes).to(o.dtype), "query_norm": dqn, "key_norm": dkn}
+    g["states"] = (rows(dk).float() @ weight("key").t() + rows(dv).float() @ weight("value").t()).reshape(s.shape)
+    like = dict(p, states=s)
+    g = {n: t.to(torch.float32 if like[n].dtype == torch.float16 else like[n].dtype) for n, t in g.items()}
+    de = d_nodes + (rows(dq).float() @ weight("query").t()).reshape(x.shape)
     # the table's rows: one product with the features' indicator (a fixed order of sums, unlike a scatter)
     hot = (rows(f[..., None]) == torch.arange(table[0], device=f.device)).to(torch.float32)
     emb = torch.zeros(table, device=f.device, dtype=torch.float32)

@@ -1,0 +1,107 @@
+"""The conditional flow's edges: states in 16 bits, what lies behind lengths and masks, empty batches and contexts, feature
+shapes and ids, and the embedding's table across streams."""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+if not torch.cuda.is_available():
+    pytest.skip("needs a ROCm GPU", allow_module_level=True)
+
+from ecnf_amd import CONFIGS, init_params  # noqa: E402
+from ecnf_amd import cnf as F  # noqa: E402
+from ecnf_amd import context as C  # noqa: E402
+from ecnf_amd import train as TR  # noqa: E402
+from ecnf_amd.engine import EcnfHandle  # noqa: E402
+
+from test_gpu_context_flow import CTX, build, features, make_context, plain  # noqa: E402
+
+HALF = {torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}
+
+
+def rel(a, b):
+    """|a - b| / |b|, Euclidean, in 64 bits"""
+    return float((a.double() - b.double()).norm() / b.double().norm())
+
+
+def reference(emb, f, ctx, dn):
+    """The embeddings and every gradient of sum(dn * node_embedding), by autograd through the plain 64-bit form."""
+    leaf = lambda t: t.detach().double().requires_grad_(True)   # noqa: E731
+    p, e, s = {n: leaf(t) for n, t in ctx.params.items()}, leaf(emb), leaf(ctx.states)
+    out = plain(e, f, ctx._replace(params=p, states=s))
+    (out * dn.double()).sum().backward()
+    return out.detach(), dict({n: t.grad for n, t in p.items()}, embedding=e.grad, states=s.grad)
+
+
+def case(contexts, length, dtype, B=6, seed=4):
+    cfg = CONFIGS["aldp"]
+    g = torch.Generator(device="cuda")
+    g.manual_seed(seed)
+    emb = torch.randn((cfg.n_features, cfg.hidden), generator=g, device="cuda")
+    f = torch.randint(0, cfg.n_features, (B, cfg.n_nodes), generator=g, device="cuda", dtype=torch.int32)
+    ctx = make_context(cfg, contexts, length, seed=seed, dtype=dtype)
+    n = torch.linspace(length / 2, length, contexts, device="cuda").to(torch.int32)
+    return cfg, g, emb, f, ctx._replace(lengths=n)
+
+
+# ------------------------------------------------------------------------------------------------ states in 16 bits
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=str)
+@pytest.mark.parametrize("size", [1.0, 1e-6, 5e-9])
+@pytest.mark.parametrize("contexts,length", [(1, 40), (6, 33)])
+def test_gradients_of_16_bit_states(contexts, length, size, dtype):
+    """The gradient of a mean loss over a batch is 1e-6 and less, below fp16's smallest number at the end: the gradients
+    keep their size whatever that of the nodes' is.  At most 16 roundings lie between the inputs and a gradient (x, its
+    weights, q, k, v, their turned forms, P, o, do, dP's P, dS, dq, dk, dv and the turned-back ones), each at most u of what
+    it rounds, in norm u / sqrt(3) and independent, and dS is a difference of two terms that are at most twice its size:
+    2 sqrt(16 / 3) u = 4.6 u, so 8 u."""
+    cfg, g, emb, f, ctx = case(contexts, length, dtype)
+    nodes, saved = C.node_embedding(emb, f, ctx, cfg, return_saved=True)
+    dn = size * torch.randn(nodes.shape, generator=g, device="cuda")
+    ref, want = reference(emb, f, ctx, dn)
+    e = emb[f.long()].double()
+    assert rel(nodes - e, ref - e) <= 8 * HALF[dtype]
+    got = C.node_embedding_grad(dn, saved)
+    assert got["states"].dtype == (torch.float32 if dtype == torch.float16 else dtype)
+    off = {n: rel(got[n], w) for n, w in want.items()}
+    print(dtype, size, {n: f"{v / HALF[dtype]:.2f} u" for n, v in off.items()}, flush=True)
+    assert max(off.values()) <= 8 * HALF[dtype], off
+
+
+def test_gradients_of_fp16_parameters():
+    """Parameters in fp16 themselves: their gradients come in fp32, a loss's size of 5e-9 included."""
+    cfg, g, emb, f, ctx = case(1, 40, torch.float32)
+    ctx = ctx._replace(params={n: p.half() for n, p in ctx.params.items()})
+    nodes, saved = C.node_embedding(emb, f, ctx, cfg, return_saved=True)
+    dn = 5e-9 * torch.randn(nodes.shape, generator=g, device="cuda")
+    got = C.node_embedding_grad(dn, saved)
+    for n, w in reference(emb, f, ctx, dn)[1].items():
+        assert got[n].dtype == torch.float32 and rel(got[n], w) <= 1e-5, n   # fp32 throughout
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=str)
+def test_training_gradients_of_16_bit_states(dtype):
+    """A training step of 1024 clusters on one shared context: the loss's own node gradients (1e-8) reach every parameter."""
+    cnf = build("lj13")
+    cfg = cnf.cfg
+    params = torch.as_tensor(F.flatten_params(init_params(cfg, 6), cfg), device="cuda")
+    g = torch.Generator(device="cuda")
+    g.manual_seed(6)
+    B = 1024
+    x1, x0 = cnf.sample_base(g, B) * 1.5, cnf.sample_base(g, B)
+    t = torch.rand(B, generator=g, device="cuda")
+    f = features(cfg)[None].expand(B, -1).contiguous()
+    ctx = make_context(cfg, 1, 64, dtype=dtype)._replace(lengths=None)
+    grads = []
+    for c in (ctx, ctx._replace(states=ctx.states.float())):
+        _, info, grad = TR.flow_matching_loss_fn(cnf, params, x1, None, f, x0=x0, t=t, with_grad=True, context=c)
+        grads.append(dict(info["context_grad"], embedding=grad[-cfg.n_features * cfg.hidden:]))
+    # 13 atoms of one feature: their rows differ by their positions only, so the scores' gradients (query, key) are sums that
+    # cancel; the values' and outputs' do not.  As above, 8 u
+    for n in ("value", "out", "embedding"):
+        assert rel(grads[0][n], grads[1][n]) <= 8 * HALF[dtype], n
+    for n in ("query", "key", "states", "query_norm", "key_norm"):
+        assert rel(grads[0][n], grads[1][n]) <= 0.5, n
+
+
