@@ -400,13 +400,13 @@ def node_embedding_grad(d_nodes: torch.Tensor, saved) -> Dict[str, torch.Tensor]
     turn = dict(turn, q_weight=turn["q_weight"].float(), k_weight=turn["k_weight"].float())   # their gradients in fp32
     dqr, dkr, dv = cross_attention_grad(do.to(o.dtype), qr, kr, v, o, lse, **keep)
     dq, dk, dqn, dkn = qk_norm_rotary_grad(dqr, dkr, q, k, **turn)
-    x, st, on = (t.to(q.dtype) for t in (x, s, o))
-    g = {"query": rows(x).t() @ rows(dq), "key": rows(st).t() @ rows(dk), "value": rows(st).t() @ rows(dv),
-         "out": rows(on).t() @ rows(d_nodes).to(o.dtype), "query_norm": dqn, "key_norm": dkn}
-    g["states"] = (rows(dk).float() @ weight("key").t() + rows(dv).float() @ weight("value").t()).reshape(s.shape)
+    # sums over the batch: in fp32, which holds the 16-bit operands exactly, and so are those of the states
+    xf, sf, of, dq, dk, dv = (rows(t).float() for t in (x, s, o, dq, dk, dv))
+    g = {"query": xf.t() @ dq, "key": sf.t() @ dk, "value": sf.t() @ dv, "out": of.t() @ rows(d_nodes), "query_norm": dqn,
+         "key_norm": dkn, "states": (dk @ weight("key").t() + dv @ weight("value").t()).reshape(s.shape)}
     like = dict(p, states=s)
     g = {n: t.to(torch.float32 if like[n].dtype == torch.float16 else like[n].dtype) for n, t in g.items()}
-    de = d_nodes + (rows(dq).float() @ weight("query").t()).reshape(x.shape)
+    de = d_nodes + (dq @ weight("query").t()).reshape(x.shape)
     # the table's rows: one product with the features' indicator (a fixed order of sums, unlike a scatter)
     hot = (rows(f[..., None]) == torch.arange(table[0], device=f.device)).to(torch.float32)
     emb = torch.zeros(table, device=f.device, dtype=torch.float32)

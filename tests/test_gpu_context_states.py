@@ -105,3 +105,21 @@ def test_training_gradients_of_16_bit_states(dtype):
         assert rel(grads[0][n], grads[1][n]) <= 0.5, n
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=str)
+def test_fp32_parameters_get_fp32_gradients(dtype):
+    """The sums over batch and atoms that give a parameter's gradient are not rounded to the states' type: the gradient of
+    the output projection is o^T d_nodes of the o that was saved up to fp32 sums, and no product is a 16-bit number."""
+    cfg, g, emb, f, ctx = case(6, 33, dtype)
+    nodes, saved = C.node_embedding(emb, f, ctx, cfg, return_saved=True)
+    dn = torch.randn(nodes.shape, generator=g, device="cuda")
+    got = C.node_embedding_grad(dn, saved)
+    o = saved[8].double().reshape(-1, CTX.n_heads * CTX.head_dim)
+    d = dn.double().reshape(o.shape[0], -1)
+    want, size = o.t() @ d, o.abs().t() @ d.abs()
+    # rows + 1 products and sums in fp32
+    assert bool(((got["out"].double() - want).abs() <= (o.shape[0] + 1) * 2.0 ** -24 * size).all())
+    for n in ("query", "key", "value", "out"):
+        assert got[n].dtype == torch.float32
+        assert float((got[n] == got[n].to(dtype).float()).float().mean()) < 0.05, n
+
+
