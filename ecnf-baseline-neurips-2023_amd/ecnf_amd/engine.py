@@ -104,10 +104,14 @@ class EcnfHandle:
             self._set_precision(precision)
 
     def _set_embedding(self, blob) -> None:
-        # the nn.Embed table [n_features, hidden] (the last entry of the flat blob): the context operators' queries
+        # the nn.Embed table [n_features, hidden] (the last entry of the flat blob): the context operators' queries.  The
+        # weights are in place when the library returns, for calls on any stream, and so is their copy here: its stream is
+        # waited for.  The old table has no reader left (ecnf_update_params waits for the device before the weights change)
         n = self.cfg.n_features * self.cfg.hidden
-        self.embedding = torch.as_tensor(blob[-n:], device=self.device).clone().reshape(self.cfg.n_features,
-                                                                                        self.cfg.hidden)
+        e = torch.as_tensor(blob[-n:], device=self.device)
+        e = e.clone() if torch.is_tensor(blob) else e
+        torch.cuda.current_stream(self.device).synchronize()
+        self.embedding = e.reshape(self.cfg.n_features, self.cfg.hidden)
 
     def _mutated(self) -> None:
         for cb in self._on_mutate:

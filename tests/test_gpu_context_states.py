@@ -123,3 +123,45 @@ def test_fp32_parameters_get_fp32_gradients(dtype):
         assert float((got[n] == got[n].to(dtype).float()).float().mean()) < 0.05, n
 
 
+# ------------------------------------------------------------------------------------------------ streams
+class _Queued:
+    """A library whose update_params leaves 50 ms of work on the current stream behind it."""
+
+    def __init__(self, lib):
+        self._lib = lib
+
+    def __getattr__(self, name):
+        fn = getattr(self._lib, name)
+        if name != "ecnf_update_params":
+            return fn
+
+        def update(*a):
+            rc = fn(*a)
+            torch.cuda._sleep(100_000_000)
+            return rc
+        return update
+
+
+def test_the_table_is_there_on_every_stream():
+    """Weights are in place when a handle's construction or update returns, on whatever stream; so is the table."""
+    cfg = CONFIGS["aldp"]
+    blobs = [torch.as_tensor(F.flatten_params(init_params(cfg, i), cfg), device="cuda") for i in range(3)]
+    tables = [b[-cfg.n_features * cfg.hidden:].reshape(cfg.n_features, cfg.hidden) for b in blobs]
+    a, b = torch.cuda.Stream(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(a):
+        h = EcnfHandle(cfg, blobs[0].cpu().numpy(), 0)
+        assert a.query()
+    lib = h.lib
+    h.lib = _Queued(lib)
+    try:
+        for i in (1, 2, 0):
+            with torch.cuda.stream(a):
+                h.update_params(blobs[i])
+                assert a.query()
+            with torch.cuda.stream(b):
+                got = h.embedding.clone()
+            b.synchronize()
+            assert torch.equal(got, tables[i])
+    finally:
+        h.lib = lib
