@@ -201,6 +201,15 @@ def _lengths(x, n: int, most: int, like: torch.Tensor, name: str) -> Optional[to
     return x.contiguous() if x.dtype == torch.int32 else x.clamp(0, most).to(torch.int32).contiguous()
 
 
+def _mask(m, shape: Tuple[int, int], like: torch.Tensor) -> Optional[torch.Tensor]:
+    if m is None:
+        return None
+    if not (torch.is_tensor(m) and m.device == like.device and m.dtype in (torch.bool, torch.uint8)
+            and tuple(m.shape) == shape):
+        raise ValueError(f"context_mask must be a bool [{shape[0]}, {shape[1]}] tensor on {like.device}")
+    return m.contiguous()
+
+
 def _attention_operands(q, k, v, query_lengths, context_lengths, context_mask, scale):
     q = _tensor(q, "q")
     k, v = _tensor(k, "k", q), _tensor(v, "v", q)
@@ -216,12 +225,7 @@ def _attention_operands(q, k, v, query_lengths, context_lengths, context_mask, s
     q, k, v = _aligned(q), _aligned(k), _aligned(v)
     ql = _lengths(query_lengths, B, q.shape[1], q, "query_lengths")
     cl = _lengths(context_lengths, C, Lk, q, "context_lengths")
-    m = context_mask
-    if m is not None:
-        if not (torch.is_tensor(m) and m.device == q.device and m.dtype in (torch.bool, torch.uint8)
-                and tuple(m.shape) == (C, Lk)):
-            raise ValueError(f"context_mask must be a bool [{C}, {Lk}] tensor on {q.device}")
-        m = m.contiguous()
+    m = _mask(context_mask, (C, Lk), q)
     return q, k, v, ql, cl, m, float(D ** -0.5 if scale is None else scale)
 
 
@@ -304,7 +308,7 @@ class Context(NamedTuple):
     """What a batch of molecules is conditioned on.  params: :func:`init_context_params`; states [C, Lk, state_dim] in
     the dtype to compute in (C: the batch, or 1 for all of it); node_positions [N, n_axes] or [batch, N, n_axes] of the
     atoms and positions [Lk, n_axes] or [C, Lk, n_axes] of the states (the same axes); lengths [C] and mask [C, Lk] as
-    in :func:`cross_attention`."""
+    in :func:`cross_attention`: the states and positions behind them are not used, NaN included."""
     cfg: ContextConfig
     params: Mapping[str, torch.Tensor]
     states: torch.Tensor
@@ -338,6 +342,24 @@ def _project(x: torch.Tensor, w: torch.Tensor, heads: int) -> torch.Tensor:
     return (x.reshape(-1, x.shape[-1]) @ w.to(x.dtype)).reshape(x.shape[0], x.shape[1], heads, -1)
 
 
+def _without_padding(context: Context, s: torch.Tensor):
+    """(states, positions) with zeros behind the lengths and masks.  The attention does not read there, but the projections
+    and the norm do, and in the backward pass NaN times a gradient of 0 would be NaN in every parameter."""
+    pos, (n, L) = context.positions, s.shape[:2]
+    lengths, mask = _lengths(context.lengths, n, L, s, "context_lengths"), _mask(context.mask, (n, L), s)
+    if lengths is None and mask is None:
+        return s, pos
+    keep = torch.ones((n, L), dtype=torch.bool, device=s.device) if mask is None else mask.bool()
+    if lengths is not None:
+        keep = keep & (torch.arange(L, device=s.device) < lengths[:, None])
+    if torch.is_tensor(pos) and pos.is_floating_point() and pos.device == s.device:
+        if pos.dim() == 3 and pos.shape[:2] == keep.shape:
+            pos = pos.masked_fill(~keep[..., None], 0.0)
+        elif pos.dim() == 2 and pos.shape[0] == L:
+            pos = pos.masked_fill(~keep.any(0)[:, None], 0.0)
+    return s.masked_fill(~keep[..., None], 0.0), pos
+
+
 @torch.no_grad()
 def node_embedding(embedding: torch.Tensor, features, context: Context, cnf_cfg: CNFConfig,
                    return_saved: bool = False):
@@ -369,9 +391,10 @@ def node_embedding(embedding: torch.Tensor, features, context: Context, cnf_cfg:
     e = embedding[:, :H][f.clamp(0, cnf_cfg.n_features - 1)]
     e = torch.where(known, e, torch.full_like(e, float("nan")))
     x = e.to(s.dtype)
+    s, positions = _without_padding(context, s)
     q, k, v = (_project(x, p["query"], c.n_heads), _project(s, p["key"], c.n_kv_heads),
                _project(s, p["value"], c.n_kv_heads))
-    turn = dict(q_positions=context.node_positions, k_positions=context.positions, q_weight=p["query_norm"],
+    turn = dict(q_positions=context.node_positions, k_positions=positions, q_weight=p["query_norm"],
                 k_weight=p["key_norm"], axes=c.axes, theta=c.theta, eps=c.eps, interleaved=c.interleaved)
     qr, kr = qk_norm_rotary(q, k, **turn)
     keep = dict(context_lengths=context.lengths, context_mask=context.mask)

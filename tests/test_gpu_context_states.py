@@ -123,6 +123,38 @@ def test_fp32_parameters_get_fp32_gradients(dtype):
         assert float((got[n] == got[n].to(dtype).float()).float().mean()) < 0.05, n
 
 
+# ------------------------------------------------------------------------------------------------ lengths and masks
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16], ids=str)
+@pytest.mark.parametrize("contexts", [1, 6])
+def test_what_lies_behind_lengths_and_masks_is_not_read(contexts, dtype):
+    """States and their positions behind a length or a mask hold NaN and infinities: embeddings and gradients have the bits
+    that they have with zeros there."""
+    cfg, g, emb, f, ctx = case(contexts, 33, dtype)
+    mask = torch.rand((contexts, 33), generator=g, device="cuda") > 0.3
+    keep = mask & (torch.arange(33, device="cuda")[None] < ctx.lengths[:, None])
+    pos = 50 * torch.rand((contexts, 33, 3), generator=g, device="cuda")
+    dn = torch.randn((6, cfg.n_nodes, cfg.hidden), generator=g, device="cuda")
+    res = []
+    for fill in (0.0, math.nan, math.inf):
+        s = torch.where(keep[..., None], ctx.states, torch.full_like(ctx.states, fill))
+        p = torch.where(keep[..., None], pos, torch.full_like(pos, fill))
+        nodes, saved = C.node_embedding(emb, f, ctx._replace(states=s, positions=p, mask=mask), cfg, return_saved=True)
+        res.append(dict(C.node_embedding_grad(dn, saved), nodes=nodes))
+    for r in res:
+        assert all(bool(torch.isfinite(t).all()) for t in r.values())
+        assert all(torch.equal(r[n], res[0][n]) for n in r)
+        assert float(r["states"][~keep].abs().max()) == 0.0
+
+
+def test_masks_of_the_context_are_checked():
+    cfg, g, emb, f, ctx = case(6, 33, torch.float32)
+    for bad in (dict(lengths=torch.ones(5, dtype=torch.int32, device="cuda")), dict(lengths=torch.ones(6, device="cuda")),
+                dict(mask=torch.ones((6, 32), dtype=torch.bool, device="cuda")),
+                dict(mask=torch.ones((6, 33), device="cuda")), dict(mask=torch.ones((1, 33), dtype=torch.bool, device="cuda"))):
+        with pytest.raises(ValueError, match="context_"):
+            C.node_embedding(emb, f, ctx._replace(**bad), cfg)
+
+
 # ------------------------------------------------------------------------------------------------ streams
 class _Queued:
     """A library whose update_params leaves 50 ms of work on the current stream behind it."""
