@@ -18,6 +18,7 @@ Nothing here falls back to the CPU.
 from __future__ import annotations
 
 import ctypes
+import math
 import struct
 from dataclasses import dataclass
 from typing import Dict, Mapping, NamedTuple, Optional, Sequence, Tuple
@@ -337,9 +338,14 @@ def init_context_params(cfg: ContextConfig, cnf_cfg: CNFConfig, seed: int = 0, d
             "key_norm": torch.ones(cfg.head_dim, device=dev)}
 
 
+def _rows(t: torch.Tensor) -> torch.Tensor:
+    """[batch, length, ..] -> [batch * length, features] (explicit sizes: any of them may be 0)"""
+    return t.reshape(t.shape[0] * t.shape[1], math.prod(t.shape[2:]))
+
+
 def _project(x: torch.Tensor, w: torch.Tensor, heads: int) -> torch.Tensor:
     """[B, L, F] @ [F, heads * D] -> [B, L, heads, D] in x's dtype"""
-    return (x.reshape(-1, x.shape[-1]) @ w.to(x.dtype)).reshape(x.shape[0], x.shape[1], heads, -1)
+    return (_rows(x) @ w.to(x.dtype)).reshape(x.shape[0], x.shape[1], heads, w.shape[1] // heads)
 
 
 def _without_padding(context: Context, s: torch.Tensor):
@@ -371,7 +377,7 @@ def node_embedding(embedding: torch.Tensor, features, context: Context, cnf_cfg:
     H, N = _hidden(cnf_cfg), cnf_cfg.n_nodes
     s = context.states
     if not (torch.is_tensor(s) and s.device == embedding.device and s.dim() == 3 and s.shape[2] == c.state_dim
-            and s.dtype in _DTYPES and s.shape[0] >= 1):
+            and s.dtype in _DTYPES):
         raise ValueError(f"states must be a floating [contexts, length, {c.state_dim}] tensor on {embedding.device}")
     if features is None:
         raise ValueError("features must be given for the EGNN vector field (build_cnf.py:73-75)")
@@ -399,7 +405,7 @@ def node_embedding(embedding: torch.Tensor, features, context: Context, cnf_cfg:
     qr, kr = qk_norm_rotary(q, k, **turn)
     keep = dict(context_lengths=context.lengths, context_mask=context.mask)
     o, lse = cross_attention(qr, kr, v, return_lse=True, **keep)
-    nodes = e + (o.reshape(-1, o.shape[2] * o.shape[3]) @ p["out"].to(o.dtype)).float().reshape(e.shape)
+    nodes = e + (_rows(o) @ p["out"].to(o.dtype)).float().reshape(e.shape)
     if not return_saved:
         return nodes
     return nodes, (f, x, s, q, k, v, qr, kr, o, lse, turn, keep, p, embedding.shape)
@@ -411,10 +417,9 @@ def node_embedding_grad(d_nodes: torch.Tensor, saved) -> Dict[str, torch.Tensor]
     per context parameter}: the table's in fp32, the others' in their operand's dtype, but in fp32 where that is float16
     (a mean loss's gradients are 1e-8 and less, nothing in float16)."""
     f, x, s, q, k, v, qr, kr, o, lse, turn, keep, p, table = saved
-    rows = lambda t: t.reshape(t.shape[0] * t.shape[1], -1)                 # noqa: E731
     d_nodes = d_nodes.float().reshape(x.shape)
     weight = lambda n: p[n].to(s.dtype).float()   # what the forward pass multiplied by                   # noqa: E731
-    do = (rows(d_nodes) @ weight("out").t()).reshape(o.shape)
+    do = (_rows(d_nodes) @ weight("out").t()).reshape(o.shape)
     if s.dtype == torch.float16:
         # fp16 ends at 2^-24, and the loss's mean over the batch puts these gradients below (LJ13, 1024 molecules: rms
         # 6e-9).  No power of two is safe for all of the chain, since dK and dV are sums over the batch and the norm divides
@@ -424,15 +429,15 @@ def node_embedding_grad(d_nodes: torch.Tensor, saved) -> Dict[str, torch.Tensor]
     dqr, dkr, dv = cross_attention_grad(do.to(o.dtype), qr, kr, v, o, lse, **keep)
     dq, dk, dqn, dkn = qk_norm_rotary_grad(dqr, dkr, q, k, **turn)
     # sums over the batch: in fp32, which holds the 16-bit operands exactly, and so are those of the states
-    xf, sf, of, dq, dk, dv = (rows(t).float() for t in (x, s, o, dq, dk, dv))
-    g = {"query": xf.t() @ dq, "key": sf.t() @ dk, "value": sf.t() @ dv, "out": of.t() @ rows(d_nodes), "query_norm": dqn,
+    xf, sf, of, dq, dk, dv = (_rows(t).float() for t in (x, s, o, dq, dk, dv))
+    g = {"query": xf.t() @ dq, "key": sf.t() @ dk, "value": sf.t() @ dv, "out": of.t() @ _rows(d_nodes), "query_norm": dqn,
          "key_norm": dkn, "states": (dk @ weight("key").t() + dv @ weight("value").t()).reshape(s.shape)}
     like = dict(p, states=s)
     g = {n: t.to(torch.float32 if like[n].dtype == torch.float16 else like[n].dtype) for n, t in g.items()}
     de = d_nodes + (dq @ weight("query").t()).reshape(x.shape)
     # the table's rows: one product with the features' indicator (a fixed order of sums, unlike a scatter)
-    hot = (rows(f[..., None]) == torch.arange(table[0], device=f.device)).to(torch.float32)
+    hot = (_rows(f[..., None]) == torch.arange(table[0], device=f.device)).to(torch.float32)
     emb = torch.zeros(table, device=f.device, dtype=torch.float32)
-    emb[:, :x.shape[-1]] = hot.t() @ rows(de)
+    emb[:, :x.shape[-1]] = hot.t() @ _rows(de)
     g["embedding"] = emb
     return g

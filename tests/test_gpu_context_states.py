@@ -155,6 +155,22 @@ def test_masks_of_the_context_are_checked():
             C.node_embedding(emb, f, ctx._replace(**bad), cfg)
 
 
+# ------------------------------------------------------------------------------------------------ shapes
+@pytest.mark.parametrize("B,contexts,length", [(0, 1, 9), (0, 0, 9), (3, 1, 0), (3, 3, 0), (0, 1, 0)])
+def test_empty_batches_and_contexts(B, contexts, length):
+    """No molecules, or contexts without states: embeddings of that shape (the table's own rows), gradients of 0."""
+    cfg, g, emb, f, ctx = case(max(contexts, 1), 9, torch.float32, B=B)
+    ctx = ctx._replace(states=ctx.states[:contexts, :length], positions=ctx.positions[:length], lengths=None)
+    nodes, saved = C.node_embedding(emb, f, ctx, cfg, return_saved=True)
+    assert torch.equal(nodes, emb[f.long()])
+    grads = C.node_embedding_grad(torch.ones_like(nodes), saved)
+    for n, t in ctx.params.items():
+        assert grads[n].shape == t.shape and float(grads[n].abs().max()) == 0.0
+    assert grads["states"].shape == ctx.states.shape
+    count = torch.bincount(f.reshape(-1), minlength=cfg.n_features).float()
+    assert torch.equal(grads["embedding"], count[:, None].expand_as(emb).contiguous())
+
+
 # ------------------------------------------------------------------------------------------------ streams
 class _Queued:
     """A library whose update_params leaves 50 ms of work on the current stream behind it."""
