@@ -389,6 +389,8 @@ def node_embedding(embedding: torch.Tensor, features, context: Context, cnf_cfg:
     f = f.to(embedding.device).long()
     if f.dim() == 1:
         f = f[None].expand(s.shape[0], -1)
+    elif f.dim() > 1 and f.numel() % N == 0:
+        f = f.reshape(f.numel() // N, N)   # [batch, N, 1], as a call without a context takes it
     if f.dim() != 2 or f.shape[1] != N or s.shape[0] not in (1, f.shape[0]):
         raise ValueError(f"features must be [{N}] or [batch, {N}] and states of the same batch or 1, got "
                          f"{tuple(f.shape)} and {tuple(s.shape)}")

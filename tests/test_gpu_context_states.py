@@ -171,6 +171,24 @@ def test_empty_batches_and_contexts(B, contexts, length):
     assert torch.equal(grads["embedding"], count[:, None].expand_as(emb).contiguous())
 
 
+def test_feature_shapes():
+    """The shapes of feature ids that the flow takes without a context give the same with one."""
+    cnf = build("aldp")
+    cfg = cnf.cfg
+    params = init_params(cfg, 5)
+    x, t = cnf.sample_base(7, 4), torch.full((4,), 0.5, device="cuda")
+    f = features(cfg)
+    each = f[None].expand(4, -1)
+    ctx = make_context(cfg, 1, 30)._replace(lengths=None)
+    want = cnf.apply(params, x, t, f, context=ctx)
+    for shape in (each, each[..., None], each[..., None].cpu(), each.reshape(4, -1, 2)):
+        assert torch.equal(cnf.apply(params, x, t, shape), cnf.apply(params, x, t, f))
+        assert torch.equal(cnf.apply(params, x, t, shape, context=ctx), want)
+    assert torch.equal(cnf.apply(params, x[:1], t[:1], f[:, None], context=ctx), cnf.apply(params, x[:1], t[:1], f, context=ctx))
+    with pytest.raises(ValueError, match="features"):
+        cnf.apply(params, x, t, each[:, :-1], context=ctx)
+
+
 # ------------------------------------------------------------------------------------------------ streams
 class _Queued:
     """A library whose update_params leaves 50 ms of work on the current stream behind it."""
