@@ -394,7 +394,8 @@ def node_embedding(embedding: torch.Tensor, features, context: Context, cnf_cfg:
     if f.dim() != 2 or f.shape[1] != N or s.shape[0] not in (1, f.shape[0]):
         raise ValueError(f"features must be [{N}] or [batch, {N}] and states of the same batch or 1, got "
                          f"{tuple(f.shape)} and {tuple(s.shape)}")
-    # device-resident ids are not read back: an id outside the table gives NaN rows, as elsewhere on the call path
+    # device-resident ids are not read back: an id outside the table gives NaN rows, as elsewhere on the call path (and a
+    # solve, which gets the ids too, reports the molecule)
     known = ((f >= 0) & (f < cnf_cfg.n_features))[..., None]
     e = embedding[:, :H][f.clamp(0, cnf_cfg.n_features - 1)]
     e = torch.where(known, e, torch.full_like(e, float("nan")))

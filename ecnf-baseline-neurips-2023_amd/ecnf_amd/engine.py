@@ -195,15 +195,20 @@ class EcnfHandle:
             raise ValueError(f"features must have {N} entries per molecule")
         return f.reshape(batch, N).to(torch.int32).contiguous()
 
-    def _nodes(self, e, batch):
+    def _nodes(self, e, batch, feat=None):
         """Node embeddings [N, H], [1, N, H] (the same for every molecule) or [batch, N, H] -> (table [rows, hidden],
-        row ids [batch, N])."""
+        row ids [batch, N]).  feat: the ids that they were made from; an atom whose id is outside the embedding's table has
+        no row (-1, which the kernels report as they report such an id)."""
         e = pad_nodes(e, self.cfg, self.device)
         N = self.cfg.n_nodes
         if e.shape[0] not in (1, batch):
             raise ValueError(f"node_embedding must have 1 or {batch} molecules, got {e.shape[0]}")
         row = torch.arange(e.shape[0] * N, device=self.device, dtype=torch.int32).reshape(-1, N)
-        return e.reshape(-1, self.cfg.hidden), row.expand(batch, N).contiguous()
+        row = row.expand(batch, N)
+        if feat is not None:
+            f = self._feat(feat, batch)
+            row = torch.where((f >= 0) & (f < self.cfg.n_features), row, -1)
+        return e.reshape(-1, self.cfg.hidden), row.contiguous()
 
     def molecules_per_workgroup(self, with_tangent: bool = False) -> int:
         v = ctypes.c_int32()
@@ -274,10 +279,11 @@ class EcnfHandle:
         fallback (with check_status, split_f16 precision): molecules that report ECNF_E_NONFINITE (an activation
         beyond the fp16 range of the split GEMMs) are solved again on the strict-fp32 kernels and replaced; a
         molecule that is still non-finite raises.
-        node_embedding [B or 1, N, H]: takes the place of the embedded features (feat is not read)."""
+        node_embedding [B or 1, N, H]: takes the place of the embedded features; feat, where given, is only
+        checked."""
         y0 = self._f32(y0, (self.cfg.event_dim,), "y0")
         B = y0.shape[0]
-        nodes, f = (None, self._feat(feat, B)) if node_embedding is None else self._nodes(node_embedding, B)
+        nodes, f = (None, self._feat(feat, B)) if node_embedding is None else self._nodes(node_embedding, B, feat)
         e = None
         if divergence == _lib.DIV_HUTCHINSON:
             if eps is None:

@@ -189,6 +189,25 @@ def test_feature_shapes():
         cnf.apply(params, x, t, each[:, :-1], context=ctx)
 
 
+def test_device_ids_outside_the_table_are_reported():
+    """A solve with a context names bad ids as one without does; the field itself gives NaN for that molecule alone."""
+    cnf = build("aldp")
+    cfg = cnf.cfg
+    params = init_params(cfg, 5)
+    x0 = cnf.sample_base(7, 3)
+    f = features(cfg)[None].repeat(3, 1)
+    f[1, 4] = cfg.n_features
+    kw = dict(use_fixed_step_size=True, step_size=0.25)
+    for ctx in (None, make_context(cfg, 1, 30)._replace(lengths=None), make_context(cfg, 3, 30)):
+        with pytest.raises(ValueError, match="ids must lie in"):
+            F.sample_cnf(cnf, params, None, features=f, x0=x0, context=ctx, **kw)
+        for call in (F.get_log_prob, lambda cnf, params, x, key, **k: F.sample_and_log_prob_cnf(cnf, params, key, **k)):
+            with pytest.raises(ValueError, match="ids must lie in"):
+                call(cnf, params, x0, 1, features=f, approx=True, context=ctx, **kw)
+        v = cnf.apply(params, x0, torch.full((3,), 0.5, device="cuda"), f, context=ctx)
+        assert bool(torch.isnan(v[1]).all()) and bool(torch.isfinite(v[[0, 2]]).all())
+
+
 # ------------------------------------------------------------------------------------------------ streams
 class _Queued:
     """A library whose update_params leaves 50 ms of work on the current stream behind it."""
