@@ -253,6 +253,25 @@ __device__ __forceinline__ int key_count(const Att& a, int c) {
   return a.klen ? __builtin_amdgcn_readfirstlane(max(0, min(a.klen[c], a.Lk))) : a.Lk;
 }
 
+// Whether the first n keys of a context leave a row exactly one: then P is 1 whatever q and k are, and dS is 0.  By length,
+// or by the mask (0: masked): every wave counts for itself, 1024 keys at a time, and stops behind the second key, so that it
+// costs the gradients one load's latency beside those of their first tiles.
+__device__ __forceinline__ bool one_key(const uint8_t* mask, int n, int lane) {
+  if (!mask || n <= 1) return n == 1;
+  int count = 0;
+  for (int k0 = 0; k0 < n && count < 2; k0 += 1024) {
+    uint8_t m[16];
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+      const int key = k0 + 64 * j + lane;
+      m[j] = key < n ? mask[key] : (uint8_t)0;
+    }
+#pragma unroll
+    for (int j = 0; j < 16; ++j) count += __popcll(__ballot(m[j] != 0));
+  }
+  return count == 1;
+}
+
 // row r of context c -> its molecule and token (r < R)
 __device__ __forceinline__ void row_of(const Att& a, int c, int r, int& b, int& i, int& g) {
   const int t = (int)a.dG.div((uint32_t)r);
@@ -774,6 +793,7 @@ __global__ __launch_bounds__(256) ECNF_WAVES(waves(HD, sizeof(T), 4, 3)) void at
   }
   KeyStream<T, DP, Sh> ks;
   ks.init(a, c, hk, split, lds, tid);
+  const bool one = one_key(ks.mask, ks.n, l);
   Reader<T, DP> rd;
   rd.init(ks.lds0, l);
 
@@ -792,7 +812,7 @@ __global__ __launch_bounds__(256) ECNF_WAVES(waves(HD, sizeof(T), 4, 3)) void at
       dp = Ops<T>::mma(rd.frag(vat, k0, s), df[s], dp);
     }
     if (!ks.whole(t)) {
-      if (ks.n == 1) dp *= 0.f;
+      if (one) dp *= 0.f;
       const float* bias = ks.bias();
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
@@ -835,8 +855,7 @@ __global__ __launch_bounds__(256) ECNF_WAVES(waves(HD, sizeof(T), 4, 3)) void at
       for (int k = 0; k < WK; ++k) delta += part[(k * WR + wr) * 32 + (l & 31)];
     }
   }
-  // one key: P is 1 whatever q and k are, so dS is 0 and not what dP and delta differ by
-  if (ks.n == 1) delta *= 0.f;
+  if (one) delta *= 0.f;   // with dP: dS is 0 and not what the two differ by
   if (split == 0 && wk == 0 && h == 0 && r < a.R) {
     const int64_t row = ((int64_t)c * a.Hk + hk) * a.R + r;
     a.row_lse[row] = lse;
@@ -981,10 +1000,11 @@ __global__ __launch_bounds__(256) ECNF_WAVES(waves(HD, sizeof(T), 3, 2)) void at
   const int n = key_count(a, c);
   const int key = (tile * WY + wy) * 32 + (l & 31);
   const uint8_t* mask = a.mask ? a.mask + (int64_t)c * a.Lk : nullptr;
-  // (a context of one key has dP = delta = 0, as in dQ: V, which only dP reads, is taken as 0)
   const bool ok = key < n && (!mask || mask[key]);
   const char* krow = ok ? a.k + ((int64_t)c * a.ks[0] + (int64_t)key * a.ks[1] + (int64_t)hk * a.ks[2]) * e : nullptr;
-  const char* vrow = ok && n > 1 ? a.v + ((int64_t)c * a.vs[0] + (int64_t)key * a.vs[1] + (int64_t)hk * a.vs[2]) * e : nullptr;
+  // (where one key is left, dP = delta = 0, as in dQ: V, which only dP reads, is taken as 0)
+  const bool one = one_key(mask, n, l);   // (all lanes of the wave count)
+  const char* vrow = ok && !one ? a.v + ((int64_t)c * a.vs[0] + (int64_t)key * a.vs[1] + (int64_t)hk * a.vs[2]) * e : nullptr;
   const uint32_t lds0 = lds_address(lds);
   Reader<T, DP> rdr;
   rdr.init(lds0, l);
