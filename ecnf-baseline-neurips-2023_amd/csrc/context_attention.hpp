@@ -254,10 +254,11 @@ __device__ __forceinline__ int key_count(const Att& a, int c) {
 }
 
 // Whether the first n keys of a context leave a row exactly one: then P is 1 whatever q and k are, and dS is 0.  By length,
-// or by the mask (0: masked): every wave counts for itself, 1024 keys at a time, and stops behind the second key, so that it
-// costs the gradients one load's latency beside those of their first tiles.
-__device__ __forceinline__ bool one_key(const uint8_t* mask, int n, int lane) {
+// or by the mask (0: masked), where `some` is a ballot of keys that the wave knows to be allowed: two of them and the answer
+// is there.  Else every wave counts for itself, 1024 keys at a time, until the second key.
+__device__ __forceinline__ bool one_key(const uint8_t* mask, int n, int lane, uint64_t some) {
   if (!mask || n <= 1) return n == 1;
+  if (__popcll(some) > 1) return false;
   int count = 0;
   for (int k0 = 0; k0 < n && count < 2; k0 += 1024) {
     uint8_t m[16];
@@ -793,7 +794,8 @@ __global__ __launch_bounds__(256) ECNF_WAVES(waves(HD, sizeof(T), 4, 3)) void at
   }
   KeyStream<T, DP, Sh> ks;
   ks.init(a, c, hk, split, lds, tid);
-  const bool one = one_key(ks.mask, ks.n, l);
+  const uint8_t first = ks.mask && l < ks.n ? ks.mask[l] : (uint8_t)0;
+  bool one = false;
   Reader<T, DP> rd;
   rd.init(ks.lds0, l);
 
@@ -825,6 +827,7 @@ __global__ __launch_bounds__(256) ECNF_WAVES(waves(HD, sizeof(T), 4, 3)) void at
     for (int x = 0; x < 16; ++x) p[x] = __builtin_amdgcn_exp2f(fmaf(p[x], sc, shift));
   };
   ks.start();
+  one = one_key(ks.mask, ks.n, l, __ballot(first != 0));   // (behind the start's own wait for mask bytes)
   // A context of one tile: delta = sum_j P dP over its keys instead of sum_d dO O.  With few keys dP - delta cancels,
   // and O was rounded (bf16: dQ and dK of 2-key rows 2.6e-3 off, so 1.7e-3, which is their own rounding); with many, O is
   // an average and its rounding is small beside dP.  The scores are made twice: nothing for 16-bit types (fp32's O is
@@ -1003,7 +1006,8 @@ __global__ __launch_bounds__(256) ECNF_WAVES(waves(HD, sizeof(T), 3, 2)) void at
   const bool ok = key < n && (!mask || mask[key]);
   const char* krow = ok ? a.k + ((int64_t)c * a.ks[0] + (int64_t)key * a.ks[1] + (int64_t)hk * a.ks[2]) * e : nullptr;
   // (where one key is left, dP = delta = 0, as in dQ: V, which only dP reads, is taken as 0)
-  const bool one = one_key(mask, n, l);   // (all lanes of the wave count)
+  const uint64_t own = __ballot(ok && l < 32);
+  const bool one = own && one_key(mask, n, l, own);
   const char* vrow = ok && !one ? a.v + ((int64_t)c * a.vs[0] + (int64_t)key * a.vs[1] + (int64_t)hk * a.vs[2]) * e : nullptr;
   const uint32_t lds0 = lds_address(lds);
   Reader<T, DP> rdr;
