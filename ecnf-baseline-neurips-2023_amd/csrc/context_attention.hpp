@@ -418,6 +418,10 @@ __device__ __forceinline__ typename Ops<T>::Frag frag_global(const char* row, in
   return f;
 }
 
+// |scale| in log2 units.  0 becomes the smallest number, under which any finite score is at most 5e-7 (a factor of 0 would
+// make NaN of a masked key's -inf)
+__device__ __forceinline__ float log2_scale(float scale) { return fmaxf(fabsf(scale) * kLog2e, 0x1p-149f); }
+
 template <class T>
 __device__ __forceinline__ void store4(char* p, f32x4 v) {
   typename Ops<T>::Quad o;
@@ -538,8 +542,7 @@ __global__ __launch_bounds__(256) ECNF_WAVES(waves(HD, sizeof(T), 4, 4)) void at
   const int hk = id % a.Hk, c = id / a.Hk;
 
   const int r = tile * kRows + wr * 32 + (l & 31);
-  // a negative scale turns the queries (exact); 0 becomes a scale under which every score rounds to 0
-  const float sc = fmaxf(fabsf(a.scale) * kLog2e, 1e-30f);
+  const float sc = log2_scale(a.scale);   // a negative scale turns the queries (exact)
   int b = 0, i = 0, g = 0;
   bool live = r < a.R;
   if (live) {
@@ -564,7 +567,7 @@ __global__ __launch_bounds__(256) ECNF_WAVES(waves(HD, sizeof(T), 4, 4)) void at
 #pragma unroll
   for (int d = 0; d < ND; ++d) o[d] = f32x16{};
   const bool idle = tile * kRows + wr * 32 >= a.R;
-  const float slack = 8.f / sc;   // P may reach 2^8 before the running maximum moves (a rescale of O less often)
+  const float slack = fminf(8.f / sc, 1e38f);   // P may reach 2^8 before the running maximum moves (a rescale of O less often)
   ks.start();
   auto step = [&](int t, auto which) {
     constexpr int cur = decltype(which)::value;
@@ -785,8 +788,7 @@ __global__ __launch_bounds__(256) ECNF_WAVES(waves(HD, sizeof(T), 4, 3)) void at
     for (int x = 0; x < 8; ++x) delta = fmaf((float)df[s][x], (float)of[x], delta);
   }
   delta = sum_halves(delta);
-  // (a scale of 0 would make NaN of a masked key's -inf)
-  const float sc = a.scale == 0.f ? 1e-30f : a.scale * kLog2e, sg = a.scale < 0.f ? -1.f : 1.f;
+  const float sg = a.scale < 0.f ? -1.f : 1.f, sc = sg * log2_scale(a.scale);
   float lse = kInf;
   if (live) {
     lse = a.lse[((int64_t)b * a.Hq + hq) * a.Lq + i] * kLog2e;
@@ -1039,7 +1041,7 @@ __global__ __launch_bounds__(256) ECNF_WAVES(waves(HD, sizeof(T), 3, 2)) void at
   const int nt = tile * WY * 32 < n ? (a.R + kRows - 1) / kRows : 0, share = (nt + a.splits - 1) / a.splits;
   const int t0 = min(split * share, nt), t1 = min(t0 + share, nt);
   const int64_t row0 = ((int64_t)c * a.Hk + hk) * a.R;
-  const float sc = a.scale * kLog2e;
+  const float sc = copysignf(log2_scale(a.scale), a.scale);
 
   float* const stats = reinterpret_cast<float*>(lds + Sh::kStat);
   const bool idle = (tile * WY + wy) * 32 >= n;

@@ -60,3 +60,57 @@ def test_one_key_left_by_a_mask(C, dtype, rows, Lk, D):
     assert float(dq[2].abs().max()) > 0.0 and float(dv[one].abs().max()) > 0.0
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=ids)
+@pytest.mark.parametrize("rows", [20, 200])
+def test_few_keys_left_by_a_mask(C, dtype, rows):
+    """Two or three keys of a context of one tile: dP - delta cancels, but dQ and dK stay as exact as their own rounding
+    and that of dS: two roundings of at most u, in norm u / sqrt(3) each, none amplified (1.5 for their spread)."""
+    g = gen(32)
+    q, do = normal(g, 64, rows, 2, 64, dtype=dtype), normal(g, 64, rows, 2, 64, dtype=dtype)
+    k, v = normal(g, 64, 60, 2, 64, dtype=dtype), normal(g, 64, 60, 2, 64, dtype=dtype)
+    kw = dict(context_mask=chosen(g, 64, 60, [2 + c % 2 for c in range(64)]))
+    want = O.attention(q, k, v, out_grad=do, **kw)
+    out, lse = C.cross_attention(q, k, v, return_lse=True, **kw)
+    u = O.half_step(dtype)
+    for name, got in zip(("dq", "dk", "dv"), C.cross_attention_grad(do, q, k, v, out, lse, **kw)):
+        O.check(name, got, *want[name])
+        off = float((got.double() - want[name][0]).norm() / want[name][0].norm())
+        assert off <= 1.5 * math.sqrt(2.0 / 3.0) * u, (name, off)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=ids)
+@pytest.mark.parametrize("rows", [20, 200])
+def test_few_keys_left_of_a_long_context(C, dtype, rows):
+    """Two or three keys of a context of many tiles: delta comes from the rounded output, so dS = P (dP - delta) carries
+    that rounding too.  Per element it is u |dO O| summed over D, against |dS|: the derived bounds hold, and in norm the
+    sum of three roundings where the terms that cancel are at most four times dS."""
+    g = gen(33)
+    q, do = normal(g, 16, rows, 2, 64, dtype=dtype), normal(g, 16, rows, 2, 64, dtype=dtype)
+    k, v = normal(g, 16, 900, 2, 64, dtype=dtype), normal(g, 16, 900, 2, 64, dtype=dtype)
+    kw = dict(context_mask=chosen(g, 16, 900, [2 + c % 2 for c in range(16)]))
+    want = O.attention(q, k, v, out_grad=do, **kw)
+    out, lse = C.cross_attention(q, k, v, return_lse=True, **kw)
+    u = O.half_step(dtype)
+    for name, got in zip(("dq", "dk", "dv"), C.cross_attention_grad(do, q, k, v, out, lse, **kw)):
+        O.check(name, got, *want[name])
+        off = float((got.double() - want[name][0]).norm() / want[name][0].norm())
+        assert off <= math.sqrt((2.0 + 16.0) / 3.0) * u, (name, off)
+
+
+# ------------------------------------------------------------------------------------------------- scales
+@pytest.mark.parametrize("rows,keys", [(5, 40), (200, 300)])
+def test_scales_far_from_one(C, rows, keys):
+    """A scale of 0 is an average whatever the scores are, and a tiny one meets scores that make up for it."""
+    g = gen(34)
+    for size, scale in ((1e14, 0.0), (2.0 ** 52, 2.0 ** -104), (2.0 ** 52, -2.0 ** -104), (2.0 ** 60, 2.0 ** -121)):
+        q, k = size * normal(g, 2, rows, 2, 32), size * normal(g, 2, keys, 2, 32)
+        v, do = normal(g, 2, keys, 2, 32), normal(g, 2, rows, 2, 32)
+        kw = dict(scale=scale, context_lengths=torch.tensor([keys, keys // 2], device="cuda"))
+        want = O.attention(q, k, v, out_grad=do, **kw)
+        out, lse = C.cross_attention(q, k, v, return_lse=True, **kw)
+        O.check("out", out, *want["out"])
+        O.check("lse", lse, *want["lse"])
+        for name, got in zip(("dq", "dk", "dv"), C.cross_attention_grad(do, q, k, v, out, lse, **kw)):
+            O.check(name, got, *want[name])
+
+
