@@ -480,6 +480,10 @@ int build_att(const ecnf_attention* o, int what, Att* a, bool pointers) {
   auto span = [&](const int64_t* st, int d) { return st[d] * e * 256 < (1ll << 31); };
   if (o->context_length > 1 && (!span(o->k_stride, 1) || !span(o->v_stride, 1)))
     return fail(ECNF_E_UNSUPPORTED, "rows of k and v must be less than 8 MiB apart");
+  // what lies behind the last key reads as zero because it lies behind the last row's end: rows must not overlap
+  if (o->context_length > 1 && (o->k_stride[1] < o->head_dim || o->v_stride[1] < o->head_dim))
+    return fail(ECNF_E_INVALID, "rows of k and v must not overlap");
+  if (o->context_length == 1) a->ks[1] = a->vs[1] = o->head_dim;   // (one row: its stride may be anything)
   auto even = [&](const int64_t* st) {
     return (per <= 1 || o->n_queries <= 1 || st[0] == st[1] * o->n_queries) && span(st, 1) && span(st, 2);
   };

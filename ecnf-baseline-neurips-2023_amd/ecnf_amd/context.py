@@ -66,6 +66,15 @@ def _aligned(x: torch.Tensor) -> torch.Tensor:
     return x if (x.data_ptr() | a * e | b * e | c * e) % 16 == 0 else x.contiguous() if not x.is_contiguous() else x.clone()
 
 
+def _key_rows(x: torch.Tensor) -> torch.Tensor:
+    """k or v as the library takes them: aligned, and its keys neither on top of each other nor 8 MiB or more apart (a copy
+    if they are)."""
+    s = x.stride(1)
+    if x.shape[1] > 1 and not x.shape[3] <= s < (8 << 20) // x.element_size():
+        return x.contiguous()
+    return _aligned(x)
+
+
 def _stream(device: torch.device) -> int:
     """torch's current stream of the device (torch.cuda.current_stream(device).cuda_stream, without building the stream
     object: 2 us of a 10 us call)."""
@@ -223,7 +232,7 @@ def _attention_operands(q, k, v, query_lengths, context_lengths, context_mask, s
         raise ValueError(f"k must have q's head_dim {D}, got {k.shape[3]}")
     if Hk < 1 or Hq < 1 or Hq % Hk:
         raise ValueError(f"q's heads ({Hq}) must be a multiple of k's ({Hk})")
-    q, k, v = _aligned(q), _aligned(k), _aligned(v)
+    q, k, v = _aligned(q), _key_rows(k), _key_rows(v)
     ql = _lengths(query_lengths, B, q.shape[1], q, "query_lengths")
     cl = _lengths(context_lengths, C, Lk, q, "context_lengths")
     m = _mask(context_mask, (C, Lk), q)

@@ -325,7 +325,8 @@ int ecnf_qk_norm_rotary_grad(const ecnf_qk_norm* o, void* workspace, size_t work
  * A row without keys, and a query at or behind query_lengths[b], gives 0 (lse -inf) and no gradient; what memory holds
  * behind a mask or a length is not used.  heads is a multiple of kv_heads (query head h reads key head
  * h / (heads / kv_heads)); context_batch is batch, or 1: one context for the whole batch (its gradients are summed over
- * the batch).  Rows of every operand start on 16-byte boundaries. */
+ * the batch).  Rows of every operand start on 16-byte boundaries; rows of k and v (key to key) do not overlap and are less than
+ * 8 MiB apart. */
 typedef struct ecnf_attention {
   const void *q, *k, *v;      /* [batch, n_queries, heads, head_dim], [context_batch, context_length, kv_heads, ..] */
   void* out;                  /* forward: written; backward: the forward's output                                  */

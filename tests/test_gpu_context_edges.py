@@ -114,3 +114,40 @@ def test_scales_far_from_one(C, rows, keys):
             O.check(name, got, *want[name])
 
 
+# ------------------------------------------------------------------------------------------------- strides
+@pytest.mark.parametrize("dtype", TYPES, ids=ids)
+def test_rows_of_keys_far_apart(C, dtype):
+    """Rows of k and v 8 MiB and more apart (a slice of a very wide buffer): as their contiguous copies."""
+    g, e = gen(35), torch.finfo(dtype).bits // 8
+    for step in ((8 << 20) // e, (9 << 20) // e):
+        far = torch.empty(7 * step, dtype=dtype, device="cuda")
+        k, v = far.as_strided((1, 6, 2, 32), (step, step, 32, 1)), far.as_strided((1, 6, 2, 32), (step, step, 32, 1), 64)
+        for x in (k, v):
+            x.copy_(normal(g, 1, 6, 2, 32, dtype=dtype))
+        q = normal(g, 3, 5, 4, 32, dtype=dtype)
+        a = C.cross_attention(q, k, v, return_lse=True)
+        b = C.cross_attention(q, k.contiguous(), v.contiguous(), return_lse=True)
+        for x, y in zip((*a, *C.cross_attention_grad(q, q, k, v, *a)),
+                        (*b, *C.cross_attention_grad(q, q, k.contiguous(), v.contiguous(), *b))):
+            assert torch.equal(x, y)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=ids)
+@pytest.mark.parametrize("rows", [5, 200])
+def test_rows_of_keys_that_overlap(C, dtype, rows):
+    """Keys that repeat one row in memory (expanded), or slide over it: as their contiguous copies, infinities included."""
+    g = gen(36)
+    q = normal(g, 2, rows, 2, 32, dtype=dtype)
+    one = normal(g, 2, 1, 2, 32, dtype=dtype)
+    one[0, 0, 0, 3] = math.inf
+    slide = normal(g, 400, dtype=dtype).as_strided((1, 41, 1, 32), (400, 8, 32, 1))
+    for x in (one.expand(2, 70, 2, 32), one, slide):
+        k = torch.nan_to_num(x, posinf=1.0)
+        a = C.cross_attention(q, k, x, return_lse=True)
+        assert torch.equal(torch.isinf(a[0]), torch.isinf(x[:, :1].expand(2, 1, 2, 32)).expand_as(a[0]))
+        b = C.cross_attention(q, k.contiguous(), x.contiguous(), return_lse=True)
+        c = C.cross_attention(q, x.new_zeros(()).expand(x.shape) + k, x.contiguous(), return_lse=True)
+        for y, z, w in zip(a, b, c):
+            assert torch.equal(y, z) and torch.equal(y, w)
+
+
