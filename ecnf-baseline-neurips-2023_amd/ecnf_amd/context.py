@@ -86,8 +86,6 @@ def _pack(layout: struct.Struct, *values) -> bytes:
         return layout.pack(*values)
     except struct.error as e:
         raise ValueError(f"a size or axis is out of its 32-bit range ({e})") from None
-    except OverflowError:
-        raise ValueError("scale or eps is out of fp32's range") from None
 
 
 def _new(x: torch.Tensor) -> torch.Tensor:

@@ -29,14 +29,3 @@ def test_rows_of_keys_are_copied_where_the_library_refuses_them(dtype):
         assert y.is_contiguous() and y.shape == t.shape and y.data_ptr() != t.data_ptr()
 
 
-def test_numbers_beyond_their_field_are_refused():
-    """scale and eps are fp32 in the library's structures, sizes 32-bit: numbers beyond are errors of the argument."""
-    for value in (1e39, -1e300):
-        with pytest.raises(ValueError, match="out of"):
-            context._pack(context._ATTENTION, *range(1, 34), value)
-        with pytest.raises(ValueError, match="out of"):
-            context._pack(context._QK_NORM, *range(1, 37), *range(1, 10), value, 2.0)
-    with pytest.raises(ValueError, match="32-bit"):
-        context._pack(context._ATTENTION, *range(1, 25), 2 ** 31, *range(26, 34), 0.5)
-
-
