@@ -304,6 +304,7 @@ int hip_fail(hipError_t e) {
 int elem_size(int dtype) { return dtype == ECNF_DTYPE_F32 ? 4 : 2; }
 
 constexpr int64_t kMaxRows = (1ll << 31) - 1024;   // 32-bit row indices, with room for the last tile
+constexpr int64_t kMaxGrid = 1ll << 24;            // a launch has fewer than 2^32 threads, a workgroup 256
 
 bool aligned(const void* p, const int64_t* st, int n, int elem, int bytes) {
   if ((uintptr_t)p % bytes) return false;
@@ -427,7 +428,7 @@ int run_norm(const ecnf_qk_norm* o, void* ws, size_t bytes, void* stream) {
     a.part = (float*)ws;
   }
   if (!grid && !(GRAD && dw)) return ECNF_OK;
-  if (grid >= (1ll << 31)) return fail(ECNF_E_UNSUPPORTED, "too many tokens");
+  if (grid >= kMaxGrid) return fail(ECNF_E_UNSUPPORTED, "too many tokens");
   DeviceScope dev(o->device);
   if (dev.err != hipSuccess) return hip_fail(dev.err);
   const hipStream_t s = (hipStream_t)stream;
@@ -522,9 +523,8 @@ int run_att(const ecnf_attention* o, int what, void* ws, size_t bytes, void* str
   const size_t need = att_floats(a, what) * 4;
   if (need && (!ws || bytes < need || (uintptr_t)ws % 16))
     return fail(ECNF_E_INVALID, "workspace below ecnf_cross_attention_workspace_size (or not 16-byte aligned)");
-  const int64_t most = 1ll << 31;
-  if (plan_fwd(a).grid >= most || (int64_t)a.C * a.Hk * a.R * (a.D / 4) / 256 >= most - 1 ||
-      (what && (plan_dq(a).grid >= most || plan_dkv(a).grid >= most || (int64_t)a.C * a.Hk * a.Lk * (a.D / 4) / 256 >= most - 1)))
+  // (the joins' grids are smaller: what they read, splits times their outputs, is at most kPartMax floats)
+  if (what ? plan_dq(a).grid >= kMaxGrid || plan_dkv(a).grid >= kMaxGrid : plan_fwd(a).grid >= kMaxGrid)
     return fail(ECNF_E_UNSUPPORTED, "too many rows");
   DeviceScope dev(o->device);
   if (dev.err != hipSuccess) return hip_fail(dev.err);

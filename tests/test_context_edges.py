@@ -3,7 +3,7 @@ import pytest
 import torch
 
 from ecnf_amd import _lib, context
-from test_context import _attention
+from test_context import _attention, _norm
 
 
 @pytest.mark.parametrize("over", [dict(k_stride=(1024, 0, 64)), dict(v_stride=(1024, 0, 64)), dict(k_stride=(1024, 56, 64)),
@@ -29,3 +29,20 @@ def test_rows_of_keys_are_copied_where_the_library_refuses_them(dtype):
         assert y.is_contiguous() and y.shape == t.shape and y.data_ptr() != t.data_ptr()
 
 
+@pytest.mark.parametrize("over", [
+    dict(batch=2 ** 22, context_batch=2 ** 22, n_queries=1, context_length=1, heads=4, kv_heads=4),
+    dict(batch=2 ** 13, context_batch=2 ** 13, n_queries=128 * 2 ** 9, context_length=3, heads=4, kv_heads=4)])
+def test_more_workgroups_than_a_launch_takes_are_refused(over):
+    """A launch has fewer than 2^32 threads, so 2^24 workgroups of 256: refused before the first of a call's launches."""
+    lib = _lib.load()
+    args = _attention(**over)
+    assert lib.ecnf_cross_attention(args, 16, 1 << 40, None) == _lib.ECNF_E_UNSUPPORTED
+    assert lib.ecnf_cross_attention_grad(args, 16, 1 << 40, None) == _lib.ECNF_E_UNSUPPORTED
+    assert b"too many rows" in lib.ecnf_last_error()
+
+
+def test_more_workgroups_of_the_norm_than_a_launch_takes_are_refused():
+    lib = _lib.load()
+    args = _norm(batch=2 ** 12, length=2 ** 12, heads=2 ** 15)
+    assert lib.ecnf_qk_norm_rotary(args, None) == _lib.ECNF_E_UNSUPPORTED
+    assert b"too many tokens" in lib.ecnf_last_error()
