@@ -717,11 +717,16 @@ int check_nodes(const ecnf_cfg& c, const float* nodes, int32_t n_rows) {
   return ECNF_OK;
 }
 
-// G, cols: team_size's decision for this solve (G = 1: the batch path)
+#ifdef ECNF_HOST_HOOKS
+std::atomic<int> g_refuse_teams{0};   // tools/asan: cooperative launches report what a refusing driver reports
+#endif
+
+// G, cols: team_size's decision for this solve (G = 1: the batch path).  refused: whether the cooperative launch itself
+// (nothing before it) was refused
 hipError_t dispatch_integrate(const ecnf_handle* h, int NT, const SolveP& sp_in, int G, int cols, const float* y0,
                               const int32_t* feat, const float* eps, float* y1, float* dlogp, int32_t* nfe,
                               int32_t* status, int B, hipStream_t stream, const NodeTable& nodes,
-                              float* sched = nullptr) {
+                              float* sched = nullptr, bool* refused = nullptr) {
   const int M = h->cfg.mlp_width, L = h->cfg.mlp_depth, D = h->cfg.dim, P = h->prec, ix = 2 * P + NT;
   size_t lds = 0;
   SolveP sp = sp_in;
@@ -766,6 +771,15 @@ hipError_t dispatch_integrate(const ecnf_handle* h, int NT, const SolveP& sp_in,
 #undef ECNF_CALL
     return hipErrorInvalidValue;
   };
+  if (G > 1) {
+#ifdef ECNF_HOST_HOOKS
+    const hipError_t e = g_refuse_teams.load() ? hipErrorIllegalState : launch(sp);
+#else
+    const hipError_t e = launch(sp);
+#endif
+    if (refused) *refused = e == hipErrorIllegalState;
+    return e;
+  }
   const int grid = (B + net.MPW - 1) / net.MPW;
   if (!(sched && G == 1 && sp.adaptive && grid > h->ncu && chunkable(M / 32, NT, P))) return launch(sp);
   // chunked, re-dealt solve (sched_floats, redeal_kernel)
@@ -922,6 +936,14 @@ int integrate_impl(ecnf_handle* h, const ecnf_solve_opts* o, const float* y0, co
 extern "C" {
 
 int ecnf_abi_version(void) { return ECNF_ABI_VERSION; }
+
+#ifdef ECNF_HOST_HOOKS
+// sanitizer build only: cooperative launches are refused (1) or made (0)
+int ecnf_debug_refuse_teams(int refuse) {
+  g_refuse_teams = refuse;
+  return ECNF_OK;
+}
+#endif
 
 #ifdef ECNF_DEVICE_CHECKS
 // device-checked diagnostic build only: OR of the failed-check bits of every kernel since the last reset
@@ -1583,7 +1605,7 @@ int integrate_impl(ecnf_handle* h, const ecnf_solve_opts* o, const float* y0, co
   sp.resume = 0;
   // team mode decided once for this solve: one read of the handle's mode (ecnf_set_team may run concurrently)
   int cols = 0;
-  const int G = team_size(h, NT, batch, &cols, h->team_mode.load(), o->divergence);
+  const int mode = h->team_mode.load(), G = team_size(h, NT, batch, &cols, mode, o->divergence);
   const size_t need = sp.sparse1 ? pcache_floats(h, batch) : 0;
   const size_t need_s = G == 1 ? sched_floats(h, o, batch) : 0;
   // the arena pointer and size are read under arena_mu, and the lock is held through the dispatch that uses them:
@@ -1632,10 +1654,12 @@ int integrate_impl(ecnf_handle* h, const ecnf_solve_opts* o, const float* y0, co
     std::lock_guard<std::mutex> tl(h->team_mu);
     if (!h->team_ev) HIP_TRY(hipEventCreateWithFlags(&h->team_ev, hipEventDisableTiming));
     if (h->team_used && h->team_stream != stream) HIP_TRY(hipStreamWaitEvent(stream, h->team_ev, 0));
-    hipError_t e = dispatch_integrate(h, NT, sp, G, cols, y0, feat, eps, y1, dlogp, nfe, status, batch, stream, nodes);
-    if (e == hipErrorIllegalState && h->team_mode.load() == 0) {
-      // no cooperative launch here (another process holds the device's cooperative queue): in auto mode the batch
-      // path, whose results are the same bits
+    bool refused = false;
+    hipError_t e = dispatch_integrate(h, NT, sp, G, cols, y0, feat, eps, y1, dlogp, nfe, status, batch, stream, nodes, nullptr,
+                                      &refused);
+    if (refused && mode == 0) {
+      // the driver takes no cooperative launch from this process now (seen while another process that had launched
+      // cooperatively was alive): in auto mode the batch path, whose results are the same bits; a forced mode reports it
       (void)hipGetLastError();
       e = dispatch_integrate(h, NT, sp, 1, 0, y0, feat, eps, y1, dlogp, nfe, status, batch, stream, nodes);
     }

@@ -182,7 +182,8 @@ int ecnf_set_exact_form(ecnf_handle* h, int32_t form);
  * M = 64 network have a team kernel too (the tangent message and shift rows are exchanged as well), used when forced
  * and for the re-dealt solves' tail teams; the exact trace always takes the batch path.  ecnf_team_workgroups reports
  * the G a solve of `batch` molecules would use (1: the batch path; with_tangent: a Hutchinson solve).  A team whose
- * exchange times out (a member not co-resident) reports status ECNF_E_HIP for its molecule. */
+ * exchange times out (a member not co-resident) reports status ECNF_E_HIP for its molecule.  Where the driver refuses the
+ * cooperative launch, auto mode solves on the batch path (the same results) and a forced mode returns ECNF_E_HIP. */
 int ecnf_set_team(ecnf_handle* h, int32_t mode);
 int ecnf_team_workgroups(ecnf_handle* h, int32_t with_tangent, int32_t batch, int32_t* G);
 

@@ -201,6 +201,53 @@ static bool device_checks(const ecnf_cfg& c, int B) {
   return true;
 }
 
+extern "C" int ecnf_debug_refuse_teams(int refuse);   // this build only (ECNF_HOST_HOOKS)
+
+// a refused cooperative launch: auto team mode gives the batch path's bits, a forced mode reports the refusal
+static void team_checks(const ecnf_cfg& c, int B) {
+  const std::vector<float> p = random_params(c, 5);
+  ecnf_handle* h = nullptr;
+  CHECK(ecnf_create(&c, p.data(), p.size(), 0, &h) == ECNF_OK && h, "create");
+  if (!h) return;
+  const size_t n = (size_t)B * c.n_nodes * c.dim;
+  float *x = dev_alloc<float>(n), *y = dev_alloc<float>(n);
+  int32_t* feat = dev_alloc<int32_t>((size_t)B * c.n_nodes);
+  std::vector<float> hx(n);
+  std::mt19937 rng(4);
+  std::normal_distribution<float> nd(0.f, 1.f);
+  for (auto& q : hx) q = nd(rng);
+  hipMemcpy(x, hx.data(), n * sizeof(float), hipMemcpyHostToDevice);
+  ecnf_solve_opts o;
+  std::memset(&o, 0, sizeof o);
+  o.solver = ECNF_SOLVER_EULER; o.divergence = ECNF_DIV_NONE; o.t1 = 1.f; o.dt0 = 0.25f;
+  o.rtol = o.atol = 1e-5f; o.max_steps = 4096;
+  int32_t G = 0;
+  CHECK(ecnf_team_workgroups(h, 0, B, &G) == ECNF_OK && G > 1, "auto teams: %d", G);
+  auto solve = [&](int mode, bool refuse, std::vector<float>& out) {
+    CHECK(ecnf_set_team(h, mode) == ECNF_OK, "mode %d", mode);
+    hipMemset(y, 0, n * sizeof(float));
+    ecnf_debug_refuse_teams(refuse);
+    const int rc = ecnf_integrate(h, &o, x, feat, nullptr, y, nullptr, nullptr, nullptr, B, nullptr);
+    ecnf_debug_refuse_teams(0);
+    out.resize(n);
+    CHECK(hipDeviceSynchronize() == hipSuccess, "sync");
+    hipMemcpy(out.data(), y, n * sizeof(float), hipMemcpyDeviceToHost);
+    return rc;
+  };
+  std::vector<float> batch, refused, again, none;
+  CHECK(solve(1, false, batch) == ECNF_OK, "batch path");
+  CHECK(solve(0, true, refused) == ECNF_OK, "auto, refused");
+  CHECK(std::memcmp(batch.data(), refused.data(), n * sizeof(float)) == 0, "auto, refused: not the batch path's bits");
+  CHECK(solve(7, true, none) == ECNF_E_HIP, "forced, refused");
+  for (float q : none) CHECK(q == 0.f, "forced, refused: wrote %g", q);
+  CHECK(solve(1, true, again) == ECNF_OK, "teams off need no cooperative launch");
+  CHECK(std::memcmp(batch.data(), again.data(), n * sizeof(float)) == 0, "teams off, refused");
+  CHECK(solve(0, false, again) == ECNF_OK, "auto");
+  CHECK(std::memcmp(batch.data(), again.data(), n * sizeof(float)) == 0, "auto: not the batch path's bits");
+  CHECK(ecnf_destroy(h) == ECNF_OK, "destroy");
+  for (void* q : {(void*)x, (void*)y, (void*)feat}) hipFree(q);
+}
+
 // the context operators: refusals on the host; with a device also one small forward and backward pass of each
 static void context_checks(bool gpu) {
   ecnf_qk_norm n;
@@ -261,6 +308,7 @@ int main() {
     gpu += device_checks(c, 5) ? 1 : 0;
   }
   context_checks(gpu > 0);
+  if (gpu) team_checks(cfgs[3], 2);
   {
     size_t lay[16];
     for (int w = 0; w < 4; ++w) CHECK(ecnf_struct_layout(w, lay, 16) > 0, "struct layout %d", w);

@@ -14,7 +14,7 @@ SAN="-Xarch_host -fsanitize=address -Xarch_host -fno-omit-frame-pointer -Xarch_h
 FLAGS="-O1 -g --offload-arch=gfx950 -std=c++17 -fPIC -fno-slp-vectorize -mllvm -amdgpu-mfma-vgpr-form -Wno-pass-failed -Wno-unused-value -Wno-unused-result -I $ROOT/include"
 if [ $# -gt 0 ]; then PARTS=("$@"); else PARTS=("$OBJ"/ecnf_part_*.o "$OBJ"/ecnf_attention_*.o); fi
 ls "${PARTS[@]}" > /dev/null
-$HIPCC $FLAGS $SAN -DECNF_SPLIT_TU -c "$CSRC/ecnf_hip.hip" -o "$OUT/ecnf_host_asan.o" &
+$HIPCC $FLAGS $SAN -DECNF_SPLIT_TU -DECNF_HOST_HOOKS -c "$CSRC/ecnf_hip.hip" -o "$OUT/ecnf_host_asan.o" &
 $HIPCC $FLAGS $SAN -c "$CSRC/ecnf_train.hip" -o "$OUT/ecnf_train_asan.o" &
 $HIPCC $FLAGS -Xclang -target-feature -Xclang -packed-fp32-ops $SAN -c "$CSRC/ecnf_context.hip" -o "$OUT/ecnf_context_asan.o" &
 wait
