@@ -368,10 +368,10 @@ def _without_padding(context: Context, s: torch.Tensor):
     if lengths is not None:
         keep = keep & (torch.arange(L, device=s.device) < lengths[:, None])
     if torch.is_tensor(pos) and pos.is_floating_point() and pos.device == s.device:
+        if pos.dim() == 2 and pos.shape[0] == L:
+            pos = pos.expand(n, L, pos.shape[1])   # (a row may lie behind one context's length and not another's)
         if pos.dim() == 3 and pos.shape[:2] == keep.shape:
             pos = pos.masked_fill(~keep[..., None], 0.0)
-        elif pos.dim() == 2 and pos.shape[0] == L:
-            pos = pos.masked_fill(~keep.any(0)[:, None], 0.0)
     return s.masked_fill(~keep[..., None], 0.0), pos
 
 

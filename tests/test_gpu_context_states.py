@@ -140,10 +140,17 @@ def test_what_lies_behind_lengths_and_masks_is_not_read(contexts, dtype):
         p = torch.where(keep[..., None], pos, torch.full_like(pos, fill))
         nodes, saved = C.node_embedding(emb, f, ctx._replace(states=s, positions=p, mask=mask), cfg, return_saved=True)
         res.append(dict(C.node_embedding_grad(dn, saved), nodes=nodes))
-    for r in res:
+    # one row of positions for all contexts, NaN where none reads it: as with zeros there
+    p = torch.where(keep.any(0)[:, None], pos[0], torch.full_like(pos[0], math.nan))
+    s = torch.where(keep[..., None], ctx.states, torch.full_like(ctx.states, math.nan))
+    shared = [dict(C.node_embedding_grad(dn, C.node_embedding(emb, f, ctx._replace(states=s, positions=x, mask=mask), cfg,
+                                                              return_saved=True)[1])) for x in (p, torch.nan_to_num(p))]
+    assert all(torch.equal(shared[0][n], t) for n, t in shared[1].items())
+    for r in res + shared:
         assert all(bool(torch.isfinite(t).all()) for t in r.values())
-        assert all(torch.equal(r[n], res[0][n]) for n in r)
         assert float(r["states"][~keep].abs().max()) == 0.0
+    for r in res:
+        assert all(torch.equal(r[n], res[0][n]) for n in r)
 
 
 def test_masks_of_the_context_are_checked():
@@ -250,3 +257,33 @@ def test_the_table_is_there_on_every_stream():
             assert torch.equal(got, tables[i])
     finally:
         h.lib = lib
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16], ids=str)
+def test_embeddings_captured_and_replayed(dtype):
+    """The embeddings and their gradients in one graph, replayed on new inputs with eager work between, equal the eager ones."""
+    cfg, g, emb, f, ctx = case(6, 33, dtype)
+    ctx = ctx._replace(positions=50 * torch.rand((33, 3), generator=g, device="cuda"))
+    dn = torch.randn((6, cfg.n_nodes, cfg.hidden), generator=g, device="cuda")
+
+    def work():
+        nodes, saved = C.node_embedding(emb, f, ctx, cfg, return_saved=True)
+        return [nodes, *C.node_embedding_grad(dn, saved).values()]
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        work()
+    torch.cuda.current_stream().wait_stream(s)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = work()
+    for n in range(3):
+        for t in (emb, dn, ctx.states, ctx.params["query"]):
+            t.copy_(torch.randn(t.shape, generator=g, device="cuda"))
+        ctx.lengths.copy_(torch.randint(0, 34, (6,), generator=g, device="cuda", dtype=torch.int32))
+        want = [x.clone() for x in work()]
+        graph.replay()
+        torch.cuda.synchronize()
+        for x, y in zip(want, outs):
+            assert torch.equal(x, y)
+        work()
