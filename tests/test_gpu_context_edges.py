@@ -151,3 +151,57 @@ def test_rows_of_keys_that_overlap(C, dtype, rows):
             assert torch.equal(y, z) and torch.equal(y, w)
 
 
+# ------------------------------------------------------------------------------------------------- roundings
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=ids)
+@pytest.mark.parametrize("shape", [(4, 22, 8, 4, 333, 4, 64), (2, 300, 4, 2, 700, 2, 128), (64, 13, 2, 1, 64, 2, 32),
+                                   (16, 1, 8, 16, 600, 2, 128)], ids=str)
+def test_errors_are_those_of_two_roundings(C, dtype, shape):
+    """Every output is rounded once, and P (out, dv) or dS (dq, dk) before its product.  A rounding to a type of half step u
+    is uniform in a binade: u / sqrt(3) in norm, times the lower end of the value's binade over the value.  That ratio is
+    0.737 for normal values (the root of E[4^floor(log2 |x|)]), so a rounding is 0.425 u, two are 0.602 u and three 0.737 u.
+    0.67 u is half way to a third."""
+    B, Lq, Hq, Ck, Lk, Hk, D = shape
+    g = gen(37)
+    q, do = normal(g, B, Lq, Hq, D, dtype=dtype), normal(g, B, Lq, Hq, D, dtype=dtype)
+    k, v = normal(g, Ck, Lk, Hk, D, dtype=dtype), normal(g, Ck, Lk, Hk, D, dtype=dtype)
+    want = O.attention(q, k, v, out_grad=do)
+    out, lse = C.cross_attention(q, k, v, return_lse=True)
+    u = O.half_step(dtype)
+    for name, got in zip(("out", "dq", "dk", "dv"), (out, *C.cross_attention_grad(do, q, k, v, out, lse))):
+        off = float((got.double() - want[name][0]).norm() / want[name][0].norm())
+        print(shape, name, f"{off / u:.3f} u", flush=True)
+        assert off <= 0.67 * u, (name, off / u)
+
+
+# ------------------------------------------------------------------------------------------------- graphs
+@pytest.mark.parametrize("dtype", TYPES, ids=ids)
+@pytest.mark.parametrize("rows", [2, 100])
+def test_wide_heads_captured_and_replayed(C, dtype, rows):
+    """Heads of 128 take more than 64 KiB of LDS, which a launch asks for beforehand: in a capture too, and replays on new
+    inputs with eager work between them equal the eager results."""
+    g = gen(38)
+    shape = dict(q=(2, rows, 4, 128), k=(2, 1500, 2, 128), v=(2, 1500, 2, 128))
+    buf = {n: normal(g, *s, dtype=dtype) for n, s in shape.items()}
+    mask = torch.rand((2, 1500), generator=g, device="cuda") > 0.2
+
+    def work():
+        out, lse = C.cross_attention(buf["q"], buf["k"], buf["v"], return_lse=True, context_mask=mask)
+        return [out, *C.cross_attention_grad(out, buf["q"], buf["k"], buf["v"], out, lse, context_mask=mask)]
+    graph = torch.cuda.CUDAGraph()
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        work()
+    torch.cuda.current_stream().wait_stream(s)
+    with torch.cuda.graph(graph):
+        outs = work()
+    for n in range(3):
+        for name in buf:
+            buf[name].copy_(normal(g, *shape[name], dtype=dtype))
+        mask.copy_(torch.rand((2, 1500), generator=g, device="cuda") > 0.2 + 0.2 * n)
+        want = [x.clone() for x in work()]
+        graph.replay()
+        torch.cuda.synchronize()
+        for x, y in zip(want, outs):
+            assert torch.equal(x, y)
+        work()

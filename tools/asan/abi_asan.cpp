@@ -310,9 +310,9 @@ int main() {
   context_checks(gpu > 0);
   if (gpu) team_checks(cfgs[3], 2);
   {
-    size_t lay[16];
-    for (int w = 0; w < 4; ++w) CHECK(ecnf_struct_layout(w, lay, 16) > 0, "struct layout %d", w);
-    CHECK(ecnf_struct_layout(9, lay, 16) == -1, "bad struct");
+    size_t lay[32];
+    for (int w = 0; w < 7; ++w) CHECK(ecnf_struct_layout(w, lay, 32) > 0, "struct layout %d", w);
+    CHECK(ecnf_struct_layout(9, lay, 32) == -1, "bad struct");
   }
   // scoped leak check of every allocation made through the library above (the ROCm runtime's own allocations are
   // suppressed by lsan.supp); run here, while the process is live, instead of at exit (leak_check_at_exit=0)
