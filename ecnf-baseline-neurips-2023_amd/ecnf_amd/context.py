@@ -352,6 +352,14 @@ def _rows(t: torch.Tensor) -> torch.Tensor:
     return t.reshape(t.shape[0] * t.shape[1], math.prod(t.shape[2:]))
 
 
+def _mm(a: torch.Tensor, b: torch.Tensor) -> torch.Tensor:
+    """a @ b in fp32.  Two 16-bit operands of a kind go to the matrix units as they are (512 x 333 states of 256: a parameter's
+    gradient 399 us of 589), their sums and the result in fp32 all the same."""
+    if a.dtype == b.dtype and a.dtype != torch.float32:
+        return torch.mm(a, b, out_dtype=torch.float32)
+    return a.float() @ b.float()
+
+
 def _project(x: torch.Tensor, w: torch.Tensor, heads: int) -> torch.Tensor:
     """[B, L, F] @ [F, heads * D] -> [B, L, heads, D] in x's dtype"""
     return (_rows(x) @ w.to(x.dtype)).reshape(x.shape[0], x.shape[1], heads, w.shape[1] // heads)
@@ -409,7 +417,9 @@ def node_embedding(embedding: torch.Tensor, features, context: Context, cnf_cfg:
     e = embedding[:, :H][f.clamp(0, cnf_cfg.n_features - 1)]
     e = torch.where(known, e, torch.full_like(e, float("nan")))
     x = e.to(s.dtype)
-    s, positions = _without_padding(context, s)
+    positions = context.positions
+    if return_saved:   # (the forward pass reads nothing behind lengths and masks)
+        s, positions = _without_padding(context, s)
     q, k, v = (_project(x, p["query"], c.n_heads), _project(s, p["key"], c.n_kv_heads),
                _project(s, p["value"], c.n_kv_heads))
     turn = dict(q_positions=context.node_positions, k_positions=positions, q_weight=p["query_norm"],
@@ -430,8 +440,8 @@ def node_embedding_grad(d_nodes: torch.Tensor, saved) -> Dict[str, torch.Tensor]
     (a mean loss's gradients are 1e-8 and less, nothing in float16)."""
     f, x, s, q, k, v, qr, kr, o, lse, turn, keep, p, table = saved
     d_nodes = d_nodes.float().reshape(x.shape)
-    weight = lambda n: p[n].to(s.dtype).float()   # what the forward pass multiplied by                   # noqa: E731
-    do = (_rows(d_nodes) @ weight("out").t()).reshape(o.shape)
+    weight = lambda n: p[n].to(s.dtype).t()   # what the forward pass multiplied by                   # noqa: E731
+    do = _mm(_rows(d_nodes), weight("out")).reshape(o.shape)
     if s.dtype == torch.float16:
         # fp16 ends at 2^-24, and the loss's mean over the batch puts these gradients below (LJ13, 1024 molecules: rms
         # 6e-9).  No power of two is safe for all of the chain, since dK and dV are sums over the batch and the norm divides
@@ -440,13 +450,14 @@ def node_embedding_grad(d_nodes: torch.Tensor, saved) -> Dict[str, torch.Tensor]
     turn = dict(turn, q_weight=turn["q_weight"].float(), k_weight=turn["k_weight"].float())   # their gradients in fp32
     dqr, dkr, dv = cross_attention_grad(do.to(o.dtype), qr, kr, v, o, lse, **keep)
     dq, dk, dqn, dkn = qk_norm_rotary_grad(dqr, dkr, q, k, **turn)
-    # sums over the batch: in fp32, which holds the 16-bit operands exactly, and so are those of the states
-    xf, sf, of, dq, dk, dv = (_rows(t).float() for t in (x, s, o, dq, dk, dv))
-    g = {"query": xf.t() @ dq, "key": sf.t() @ dk, "value": sf.t() @ dv, "out": of.t() @ _rows(d_nodes), "query_norm": dqn,
-         "key_norm": dkn, "states": (dk @ weight("key").t() + dv @ weight("value").t()).reshape(s.shape)}
+    # the sums over the batch in fp32; the states' two products as one, rounded once
+    xt, st, ot, dq, dk, dv = _rows(x).t(), _rows(s).t(), _rows(o).t(), _rows(dq), _rows(dk), _rows(dv)
+    g = {"query": _mm(xt, dq), "key": _mm(st, dk), "value": _mm(st, dv), "out": _mm(ot, _rows(d_nodes)), "query_norm": dqn,
+         "key_norm": dkn,
+         "states": (torch.cat((dk, dv), 1) @ torch.cat((weight("key"), weight("value"))).to(dk.dtype)).reshape(s.shape)}
     like = dict(p, states=s)
     g = {n: t.to(torch.float32 if like[n].dtype == torch.float16 else like[n].dtype) for n, t in g.items()}
-    de = d_nodes + (dq @ weight("query").t()).reshape(x.shape)
+    de = d_nodes + _mm(dq, weight("query")).reshape(x.shape)
     # the table's rows: one product with the features' indicator (a fixed order of sums, unlike a scatter)
     hot = (_rows(f[..., None]) == torch.arange(table[0], device=f.device)).to(torch.float32)
     emb = torch.zeros(table, device=f.device, dtype=torch.float32)
