@@ -19,8 +19,8 @@
 //
 // Types: bf16, fp16 (one 32x32x16 instruction a step) and fp32 (eight 32x32x2 instructions on the same fragments: the
 // k order inside a step is free as long as A and B agree).  Scores, softmax statistics and all accumulators are fp32;
-// P and dS are rounded to the operand type for the second products (half a step of the type, 2^-9 / 2^-12 relative,
-// independent from key to key, so it averages in the sums).
+// P and dS are rounded to the operand type for the second products (at most half a step, 2^-8 / 2^-11 relative, independent
+// from key to key: with the outputs' own rounding 0.6 half steps in norm, where one rounding is 0.43).
 #pragma once
 #include <hip/hip_runtime.h>
 
@@ -38,8 +38,8 @@ typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
 // waves a SIMD: at least LOW (what the kernel's registers allow without spills); at head_dim 128 exactly that many, so
-// that the scheduler spends the registers on reads ahead (long bf16 forward 1031 -> 1023 us), and elsewhere as many as
-// fit (at head_dim 64 three instead of four make the 333-key forward 40 us of 35)
+// that the scheduler spends the registers on reads ahead (long bf16 forward 1078 us, with as many as fit 1085), and
+// elsewhere as many as fit (training pass of 22 x 129 at head_dim 16, exactly LOW: fp32 82 us for 74, bf16 46 for 43)
 #define ECNF_WAVES(LOW) __attribute__((amdgpu_waves_per_eu((LOW), HD <= 64 ? 8 : (LOW))))
 constexpr int waves(int hd, int bytes, int at32, int at64) {
   return bytes == 4 ? (hd <= 32 ? 3 : hd <= 64 ? 2 : 1) : hd <= 32 ? at32 : hd <= 64 ? at64 : 2;
@@ -142,7 +142,7 @@ __device__ __forceinline__ float sum_halves(float x) {
 // The backward pass in fp16.  P is about 1 / keys and dS smaller still, at or below fp16's subnormals in long contexts
 // (1 / 16384 = 2^-14).  So P is made as 2^14 P (at most 2^14: a shift of the exponent's argument, for nothing), dS with
 // it, and where the largest 2^14 |dS| of a column (row of dQ, key of dK) so far is not in [1, 2^15] the column is scaled
-// by a power of two besides, which its accumulators carry.  What is rounded away is then 2^-12 of the value, or 2^-25 of
+// by a power of two besides, which its accumulators carry.  What is rounded away is then 2^-11 of the value, or 2^-25 of
 // the column's largest.  Other types have fp32's exponents and need nothing.
 template <class T>
 struct Range {
@@ -830,10 +830,11 @@ __global__ __launch_bounds__(256) ECNF_WAVES(waves(HD, sizeof(T), 4, 3)) void at
   };
   ks.start();
   one = one_key(ks.mask, ks.n, l, __ballot(first != 0));   // (behind the start's own wait for mask bytes)
-  // A context of one tile: delta = sum_j P dP over its keys instead of sum_d dO O.  With few keys dP - delta cancels,
-  // and O was rounded (bf16: dQ and dK of 2-key rows 2.6e-3 off, so 1.7e-3, which is their own rounding); with many, O is
-  // an average and its rounding is small beside dP.  The scores are made twice: nothing for 16-bit types (fp32's O is
-  // exact enough; there it would cost 74 -> 79 us of the 22 x 129 training pass).
+  // A context whose length is one tile: delta = sum_j P dP over its keys instead of sum_d dO O.  With few keys dP - delta
+  // cancels, and O was rounded (bf16: dQ and dK of 2-key rows 2.6e-3 off, so 1.7e-3, which is their own rounding); with many,
+  // O is an average and its rounding is small beside dP.  (Few keys that a mask leaves of many tiles keep delta from O: to
+  // sum over them first would read all tiles twice.)  The scores are made twice: nothing for 16-bit types (fp32's O is exact
+  // enough; there it would cost 74 -> 79 us of the 22 x 129 training pass).
   if (sizeof(T) == 2 && ks.t0 < ks.t1 && ks.n <= kKeys) {
     dma_wait();
     __syncthreads();
@@ -1220,10 +1221,16 @@ inline int ceil_div(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
 //
 // The loop is split until the workgroups fill the chip once (one a CU where a row of a tile has 256 bytes or more: their
 // buffers fill its LDS; else two), but into parts of no fewer than 2 tiles (narrow), 8 (16-bit types) or 4 (fp32, whose
-// tiles take longer).  Measured, us: one token, 131072 keys of 8 x 128, bf16: one a CU 111, two 129; gradients of 22 x 1024
-// rows on 512 keys of 8 x 64, fp16: 162, two 138; 22 fp32 rows on 4 x 4096 keys of 4 x 32: parts of 4 tiles 31, of 2 27;
-// gradients of 100 rows on 2 x 4000 keys of 4 x 64, bf16: parts of 4 tiles 56, of 8 40; 300 fp32 rows on 2000 keys: 52
-// and 71.
+// tiles take longer).  Both sides measured, us, as it is | the other way:
+//   one a CU: one token, 131072 keys of 8 x 128, bf16 111 | two 129; 1000 rows on 4000 keys of 4 x 128, fp32 92 | 115 (but
+//     gradients of 256 x 22 rows on 512 shared keys of 8 x 64, fp32 297 | 275)
+//   two a CU: one token, 4 x 16384 keys of 8 x 64, bf16 29 | one 31; those gradients in fp16 74 | 77
+//   narrow: gradients of 4 rows on 16 x 2048 keys of 2 x 64, fp32 60 | parts of 4 70, of 1 60; bf16 49 | 49, 47
+//   16-bit: gradients of 256 x 22 rows on 512 shared keys of 8 x 64, bf16 70 | parts of 4 94, of 16 72; of 100 rows on
+//     2 x 4000 keys of 4 x 64, bf16 50 | 50, 71
+//   fp32: 100 rows on 2 x 4000 keys of 4 x 64 37 | parts of 8 50, of 2 34; gradients of 300 rows on 2000 keys 98 | 157, 65
+// One tile buffer for narrow parts of at most two tiles: fp32 22 x 129 training pass 74 | two 84; two buffers for more: one
+// token on 64 x 8192 keys of 8 x 128, bf16 382 | one 410.
 inline Plan make_plan(const Att& a, int outer, int inner, int narrow_step, int wide_step, int64_t per_row, bool lse) {
   Plan p;
   const int64_t pairs = (int64_t)a.C * a.Hk;

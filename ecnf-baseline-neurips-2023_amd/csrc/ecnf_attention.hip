@@ -36,8 +36,8 @@ Att with_plan(Att a, const Plan& p, float* part) {
 }
 
 // Few rows (a single token, a small molecule): the waves split the keys, with one tile buffer where a workgroup has at
-// most two tiles (fp32, 22 rows x 129 keys, forward and gradients: 89 us, with two buffers 100) and two where it has more
-// (one token x 8192 keys: 381 us, with one 408).  More rows: the waves split the rows and share every tile.
+// most two tiles and two where it has more (make_plan has both measured).  More rows: the waves split the rows and share
+// every tile.
 #if !ECNF_ATT_GRAD
 template <int HD>
 hipError_t fwd(const Att& in, hipStream_t s) {
