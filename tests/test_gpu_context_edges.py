@@ -151,6 +151,46 @@ def test_rows_of_keys_that_overlap(C, dtype, rows):
             assert torch.equal(y, z) and torch.equal(y, w)
 
 
+# ------------------------------------------------------------------------------------------------- groups and widths
+@pytest.mark.parametrize("dtype", TYPES, ids=ids)
+@pytest.mark.parametrize("shape", [(3, 17, 6, 3, 70, 2, 32), (4, 9, 15, 1, 300, 3, 64), (2, 40, 36, 2, 33, 3, 16),
+                                   (3, 1, 14, 3, 500, 2, 128), (5, 50, 5, 1, 130, 1, 8), (2, 3, 300, 1, 90, 1, 16),
+                                   (2, 65, 2, 2, 200, 2, 56), (2, 64, 2, 2, 200, 2, 104)], ids=str)
+@pytest.mark.parametrize("masked", [False, True])
+def test_groups_that_do_not_divide_a_tile(C, dtype, shape, masked):
+    """Query heads a key head of 3, 5, 7, 12 and 300, and widths between the compiled ones: rows of a token cross tiles."""
+    B, Lq, Hq, Ck, Lk, Hk, D = shape
+    g = gen(39)
+    q, do = normal(g, B, Lq, Hq, D, dtype=dtype), normal(g, B, Lq, Hq, D, dtype=dtype)
+    k, v = normal(g, Ck, Lk, Hk, D, dtype=dtype), normal(g, Ck, Lk, Hk, D, dtype=dtype)
+    kw = {}
+    if masked:
+        kw = dict(context_mask=torch.rand((Ck, Lk), generator=g, device="cuda") > 0.5,
+                  query_lengths=torch.randint(0, Lq + 1, (B,), generator=g, device="cuda"),
+                  context_lengths=torch.randint(1, Lk + 1, (Ck,), generator=g, device="cuda"))
+    want = O.attention(q, k, v, out_grad=do, **kw)
+    out, lse = C.cross_attention(q, k, v, return_lse=True, **kw)
+    for name, got in zip(("out", "lse", "dq", "dk", "dv"), (out, lse, *C.cross_attention_grad(do, q, k, v, out, lse, **kw))):
+        O.check(name, got, *want[name])
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=ids)
+def test_queries_expanded_over_batch_length_and_heads(C, dtype):
+    """q and out_grad that repeat in memory: the bits of their contiguous copies."""
+    g = gen(40)
+    k, v = normal(g, 1, 90, 2, 32, dtype=dtype), normal(g, 1, 90, 2, 32, dtype=dtype)
+    for shape in ((1, 20, 4, 32), (5, 1, 4, 32), (5, 20, 1, 32), (1, 1, 4, 32), (1, 1, 1, 32)):
+        for full in ((5, 20, 4, 32), (5, 1, 4, 32)):
+            if any(a not in (1, b) for a, b in zip(shape, full)):
+                continue
+            q, do = normal(g, *shape, dtype=dtype).expand(full), normal(g, *shape, dtype=dtype).expand(full)
+            a = C.cross_attention(q, k, v, return_lse=True)
+            b = C.cross_attention(q.contiguous(), k, v, return_lse=True)
+            for x, y in zip((*a, *C.cross_attention_grad(do, q, k, v, *a)),
+                            (*b, *C.cross_attention_grad(do.contiguous(), q.contiguous(), k, v, *b))):
+                assert torch.equal(x, y)
+
+
 # ------------------------------------------------------------------------------------------------- roundings
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=ids)
 @pytest.mark.parametrize("shape", [(4, 22, 8, 4, 333, 4, 64), (2, 300, 4, 2, 700, 2, 128), (64, 13, 2, 1, 64, 2, 32),

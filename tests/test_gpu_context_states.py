@@ -14,7 +14,8 @@ from ecnf_amd import CONFIGS, init_params  # noqa: E402
 from ecnf_amd import cnf as F  # noqa: E402
 from ecnf_amd import context as C  # noqa: E402
 from ecnf_amd import train as TR  # noqa: E402
-from ecnf_amd.engine import EcnfHandle  # noqa: E402
+from ecnf_amd.engine import EcnfHandle, SolveOptions  # noqa: E402
+from ecnf_amd.params import CNFConfig  # noqa: E402
 
 from test_gpu_context_flow import CTX, build, features, make_context, plain  # noqa: E402
 
@@ -287,3 +288,47 @@ def test_embeddings_captured_and_replayed(dtype):
         for x, y in zip(want, outs):
             assert torch.equal(x, y)
         work()
+
+
+# ------------------------------------------------------------------------------------------------ a call's own table
+@pytest.mark.parametrize("B", [1, 2, 12])
+def test_own_table_in_team_solves(B):
+    """QM9's solves of few molecules run as teams; with a call's own table too, in every team size, bit by bit."""
+    cfg = CONFIGS["qm9"]
+    h = EcnfHandle(cfg, init_params(cfg, 1), 0)
+    g = torch.Generator(device="cuda")
+    g.manual_seed(8)
+    x = torch.randn((B, cfg.event_dim), generator=g, device="cuda")
+    f = features(cfg)
+    e = h.embedding[f.long()][None]
+    opts = SolveOptions("euler", 0.25)
+    want = h.integrate(x, f, 0.0, 1.0, opts)[0]
+    for mode in (0, 1, 4):
+        h.set_team(mode)
+        assert torch.equal(h.integrate(x, None, 0.0, 1.0, opts, node_embedding=e)[0], want)
+        assert torch.equal(h.integrate(x, f, 0.0, 1.0, opts, node_embedding=e.expand(B, -1, -1))[0], want)
+    h.set_team(0)
+    moved = e + 0.1 * torch.randn(e.shape, generator=g, device="cuda")
+    res = []
+    for mode in (0, 1):
+        h.set_team(mode)
+        res.append(h.integrate(x, None, 0.0, 1.0, opts, node_embedding=moved)[0])
+    h.set_team(0)
+    assert torch.equal(*res) and not torch.equal(res[0], want)
+
+
+def test_own_table_of_large_molecules_and_in_fp32():
+    """Molecules of more than 33 atoms (receiver-tiled edges) and the strict fp32 kernels read the table as well."""
+    big = CNFConfig(n_nodes=48, dim=3, n_features=3, hidden=64, mlp_width=128, mlp_depth=3, n_blocks=2, base_scale=1.0,
+                    sigma_min=0.01)
+    for cfg, precision in ((big, "split_f16"), (big, "fp32"), (CONFIGS["aldp"], "fp32")):
+        h = EcnfHandle(cfg, init_params(cfg, 1), 0, precision=precision)
+        g = torch.Generator(device="cuda")
+        g.manual_seed(9)
+        x = torch.randn((5, cfg.event_dim), generator=g, device="cuda")
+        f = features(cfg)
+        e = h.embedding[f.long()][None]
+        opts = SolveOptions("euler", 0.25)
+        assert torch.equal(h.integrate(x, None, 0.0, 1.0, opts, node_embedding=e)[0], h.integrate(x, f, 0.0, 1.0, opts)[0])
+        t = torch.full((5,), 0.5, device="cuda")
+        assert torch.equal(h.vector_field(x, t, node_embedding=e.expand(5, -1, -1)), h.vector_field(x, t, f))
