@@ -1,6 +1,6 @@
-// abi_asan.cpp — AddressSanitizer driver for the HOST side of libecnf_hip.so ("-fsanitize=address
-// host build").  Built by tools/asan/build.sh against an ASan-instrumented build of the host translation units
-// (the host code of ecnf_hip.hip, ecnf_train.hip and ecnf_context.hip); device code is not instrumented (no GPU ASan on this pool).
+// abi_asan.cpp — AddressSanitizer driver for the HOST side of libecnf_hip.so.  Built by tools/asan/build.sh against an
+// ASan-instrumented build of the host translation units (the host code of ecnf_hip.hip, ecnf_train.hip and
+// ecnf_context.hip; with ECNF_HOST_HOOKS); device code is not instrumented.
 //
 // Without a GPU it exercises every host path that runs before the first device call: argument checks, the
 // ravel_pytree param walk and the split / fragment repacking of ecnf_create (which then fails with ECNF_E_HIP).

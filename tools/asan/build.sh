@@ -1,5 +1,5 @@
 #!/bin/bash
-# AddressSanitizer build of the host side of libecnf_hip.so (SURVEY.md section 5) and of its driver abi_asan.cpp.
+# AddressSanitizer build of the host side of libecnf_hip.so and of its driver abi_asan.cpp.
 # The host translation units (ecnf_hip.hip, ecnf_train.hip and ecnf_context.hip host code) are instrumented on the HOST pass only
 # (-Xarch_host); device code is not.  The per-shape kernel objects are the product build's (run
 # __graft_entry__.build() first; it passes the exact object list as arguments, else every ecnf_part_*.o and ecnf_attention_*.o of the build
